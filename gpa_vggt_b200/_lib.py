@@ -68,6 +68,14 @@ SIGNATURES = {
                                   _vp, _c_int, _c_f32, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _vp]),
     "gpa_frame_pool": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,
                                 _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp]),
+    "gpa_residual_norm": (_c_int, [_vp, _c_int, _c_i64, _vp, _c_int, _c_i64, _vp, _c_int, _c_i64, _c_int,
+                                   _c_int, _c_int, _vp, _vp, _c_f32, _c_int, _vp, _vp, _c_int, _c_f32, _vp,
+                                   _c_i64, _vp, _c_i64, _vp, _vp]),
+    "gpa_residual_norm_backward_workspace_bytes": (_c_i64, [_c_int, _c_int, _c_i64]),
+    "gpa_residual_norm_backward": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_int, _c_i64, _vp, _c_int,
+                                            _c_i64, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp,
+                                            _vp, _c_int, _vp, _c_int, _vp, _c_i64, _vp, _c_i64, _vp, _vp,
+                                            _vp, _vp, _vp, _vp, _c_i64, _vp]),
     "gpa_lse_combine": (_c_int, [_c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _vp]),
 }

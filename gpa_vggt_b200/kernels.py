@@ -5,6 +5,7 @@ launch on the current stream.  One function per entry point of
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
@@ -525,6 +526,176 @@ def residual_scale(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     call("gpa_residual_scale_bf16", ptr(x2), x2.stride(0), ptr(y2), y2.stride(0), ptr(g), x2.shape[0], C,
          ptr(o2), o2.stride(0), stream_of(x))
     return out
+
+
+_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+
+
+def _device_of(*tensors, what: str):
+    """The one CUDA device of the given tensors."""
+    require_cuda(*tensors, what=what)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"{what}: tensors are on different devices")
+    return devices.pop()
+
+
+def _on(device):
+    """Make `device` current for a launch on one of its streams."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """[rows, cols] with 16-byte aligned rows (a view where t allows it)."""
+    t2 = t.reshape(t.numel() // cols, cols)
+    if t2.stride(-1) != 1 or t2.stride(0) % 8 or not aligned(t2):
+        t2 = t2.contiguous()
+        if not aligned(t2):
+            t2 = t2.clone()
+    return t2
+
+
+def _ld(t2: torch.Tensor) -> int:
+    """Row stride of _rows' result (a single row's stride says nothing)."""
+    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
+
+
+def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and 16-byte aligned."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if aligned(t) else t.clone()
+
+
+def _residual_norm_launch(x, y, gate, weight, bias, post_weight, post_bias, eps, kind, post_kind, post_eps,
+                          want_stats):
+    C = x.shape[-1]
+    rows = x.numel() // C
+    z = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = None if kind is None else torch.empty(x.shape, device=x.device, dtype=y.dtype)
+    stats = torch.empty(rows, 4, device=x.device, dtype=F32) if want_stats else None
+    if rows == 0:
+        return z, h, stats
+    x2, y2, gate = _rows(x, C), _rows(y, C), _param(gate)
+    weight, bias, post_weight, post_bias = (_param(t) for t in (weight, bias, post_weight, post_bias))
+    first = next((t for t in (weight, bias, post_weight, post_bias) if t is not None), None)
+    with _on(x.device):
+        call("gpa_residual_norm", ptr(x2), _dt(x), _ld(x2), ptr(y2), _dt(y), _ld(y2), ptr(gate),
+             0 if gate is None else _dt(gate), 0 if gate is None else rows // (gate.numel() // C), rows, C,
+             _NORM_KINDS[post_kind], ptr(post_weight), ptr(post_bias), post_eps, _NORM_KINDS[kind],
+             ptr(weight), ptr(bias), 0 if first is None else _dt(first), eps, ptr(z), C, ptr(h), C, ptr(stats),
+             stream_of(x))
+    return z, h, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """residual_norm with gradients: keeps z, y and each row's statistics."""
+
+    @staticmethod
+    def forward(ctx, x, y, gate, weight, bias, post_weight, post_bias, eps, kind, post_kind, post_eps):
+        z, h, stats = _residual_norm_launch(x, y, gate, weight, bias, post_weight, post_bias, eps, kind,
+                                            post_kind, post_eps, True)
+        ctx.kinds = (kind, post_kind)
+        # the norms' own biases enter no gradient but their types do
+        ctx.save_for_backward(z, y, gate, weight, bias, post_weight, post_bias, stats)
+        ctx.set_materialize_grads(False)
+        return z if h is None else (z, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dz, dh=None):
+        z, y, gate, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
+        kind, post_kind = ctx.kinds
+        C = z.shape[-1]
+        rows = z.numel() // C
+        params = (gate, weight, bias, post_weight, post_bias)
+        if (dz is None and dh is None) or rows == 0:
+            return (*(None if t is None else torch.zeros_like(t) for t in (z, y, *params)),
+                    None, None, None, None)
+        if dz is not None:
+            dz = _rows(dz, C)
+        if dh is not None:
+            dh = _rows(dh, C)
+        y2, gate_c = _rows(y, C), _param(gate)
+        dx, dy = torch.empty_like(z), torch.empty(y.shape, device=y.device, dtype=y.dtype)
+        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if t is not None and need else None
+                 for t, need in zip(params, ctx.needs_input_grad[2:7])]
+        gate_rows = rows if gate is None else rows // (gate.numel() // C)
+        first = next((t for t in params[1:] if t is not None), None)
+        weight, post_weight, post_bias = _param(weight), _param(post_weight), _param(post_bias)
+        size = _lib.load().gpa_residual_norm_backward_workspace_bytes(rows, C, gate_rows)
+        ws = torch.empty(size, device=z.device, dtype=torch.uint8)
+        with _on(z.device):
+            call("gpa_residual_norm_backward", ptr(dz), 0 if dz is None else _ld(dz), ptr(dh),
+                 0 if dh is None else _ld(dh), ptr(z), _dt(z), C, ptr(y2), _dt(y), _ld(y2), ptr(stats),
+                 ptr(gate_c), 0 if gate is None else _dt(gate), gate_rows, rows, C, _NORM_KINDS[post_kind],
+                 ptr(post_weight), ptr(post_bias), _NORM_KINDS[kind], ptr(weight),
+                 0 if first is None else _dt(first), ptr(dx), C, ptr(dy), C, *(ptr(t) for t in grads), ptr(ws),
+                 size, stream_of(z))
+        return (dx, dy, *grads, None, None, None, None)
+
+
+def _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind, post_kind):
+    if x.dim() < 1 or x.shape != y.shape:
+        raise ValueError("residual_norm: x and y must have one shape [..., C]")
+    if (x.dtype, y.dtype) not in ((BF16, BF16), (F32, BF16), (F32, F32)):
+        raise TypeError("residual_norm: x and y must be bf16 or fp32, y no wider than x")
+    C = x.shape[-1]
+    if C < 8 or C % 8 or C > 8192:
+        raise ValueError("residual_norm: the last dim must be a multiple of 8, at most 8192")
+    if x.numel() // C >= 2 ** 31:
+        raise ValueError("residual_norm: fewer than 2^31 rows required")
+    if kind not in _NORM_KINDS or post_kind not in _NORM_KINDS:
+        raise ValueError("residual_norm: kind and post_kind are None, 'layer' or 'rms'")
+    if (kind is None and (weight is not None or bias is not None)) or (
+            post_kind is None and (post_weight is not None or post_bias is not None)):
+        raise ValueError("residual_norm: parameters of a norm that is off")
+    params = [t for t in (weight, bias, post_weight, post_bias) if t is not None]
+    if any(tuple(t.shape) != (C,) for t in params):
+        raise ValueError("residual_norm: norm weights and biases must be [C]")
+    if any(t.dtype not in (F32, BF16) or t.dtype != params[0].dtype for t in params):
+        raise TypeError("residual_norm: norm weights and biases must all be bf16 or all fp32")
+    if gate is not None:
+        if gate.dtype not in (F32, BF16):
+            raise TypeError("residual_norm: gate must be bf16 or fp32")
+        lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
+        n = len(lead)
+        while n and lead[n - 1] == 1:
+            n -= 1
+        if gate.dim() < 1 or gate.shape[-1] != C or (gate.dim() > 1 and (gate.dim() != x.dim()
+                                                                        or lead[:n] != full[:n])):
+            raise ValueError("residual_norm: gate must be [C], or x's shape with trailing dims before the "
+                             "last of size 1 ([B, 1, C], [B, N, C])")
+    _device_of(x, y, gate, weight, bias, post_weight, post_bias, what="residual_norm")
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = None,
+                  weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                  eps: float = 1e-6, kind: Optional[str] = "layer", post_kind: Optional[str] = None,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  post_eps: float = 1e-6):
+    """The residual stream between two sub-blocks in one pass, with gradients:
+    z = x + gate * P(y) and h = N(z) over the last dim -> (z, h).
+
+    P is y itself (post_kind None) or its "layer" / "rms" norm with optional
+    post_weight, post_bias; N is the norm in front of the next sub-block
+    (kind, weight, bias, eps; None: no norm, and h is None).  gate is None,
+    [C] (a LayerScale), or x's shape with trailing dims before the last of size
+    1: [B, 1, C] per sequence, [B, N, C] per token.  x and z carry the stream's
+    type, y and h the branch's: bf16/bf16, fp32/bf16 or fp32/fp32; the norm
+    parameters are all bf16 or all fp32.  fp32 arithmetic; for a bf16 stream the
+    roundings are those of residual_scale and layernorm one after the other.
+    C % 8 == 0, C <= 8192.  Differentiable once in x, y, gate and the norm
+    parameters; column sums run in a fixed order."""
+    _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind, post_kind)
+    args = (x, y, gate, weight, bias, post_weight, post_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        out = _ResidualNorm.apply(*args, float(eps), kind, post_kind, float(post_eps))
+        return out if kind is not None else (out, None)
+    return _residual_norm_launch(*args, float(eps), kind, post_kind, float(post_eps), False)[:2]
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_norm, k_norm, positions: Optional[torch.Tensor],

@@ -480,8 +480,21 @@ class Block(nn.Module):
         self.ls2 = LayerScale(dim, init_values=init_values) if init_values else nn.Identity()
 
     def forward(self, x, pos=None, global_merging=None):
-        x = _residual(x, self.ls1, self.attn(self.norm1(x), pos=pos, global_merging=global_merging))
-        return _residual(x, self.ls2, self.mlp(self.norm2(x)))
+        y = self.attn(self.norm1(x), pos=pos, global_merging=global_merging)
+        x, h = _residual_norm(x, self.ls1, y, self.norm2)
+        return _residual(x, self.ls2, self.mlp(h))
+
+
+def _residual_norm(x, ls, y, norm):
+    """(x + ls(y), norm of it).  Where _residual and LayerNorm both take their
+    fused kernels this is one pass with the same results, bit for bit."""
+    C = x.shape[-1]
+    if (isinstance(ls, LayerScale) and isinstance(norm, LayerNorm) and x.is_cuda and x.dtype == BF16
+            and y.dtype == BF16 and ls.gamma.dtype == BF16 and x.shape == y.shape
+            and norm.weight is not None and norm.bias is not None and C in (256, 512, 1024, 2048)):
+        return kernels.residual_norm(x, y, ls.gamma, norm.weight, norm.bias, norm.eps)
+    x = _residual(x, ls, y)
+    return x, norm(x)
 
 
 def _residual(x, ls, y):

@@ -49,6 +49,10 @@ extern "C" {
 #define GPA_DTYPE_F32 0
 #define GPA_DTYPE_BF16 1
 
+#define GPA_NORM_NONE 0
+#define GPA_NORM_LAYER 1
+#define GPA_NORM_RMS 2
+
 /* Library version (major*10000 + minor*100 + patch). */
 GPA_API int gpa_version(void);
 
@@ -378,6 +382,47 @@ GPA_API int gpa_bias_act_bf16(const void* y, const void* bias, const void* res, 
  * evaluates it for bf16 tensors.  n % 8 == 0, 16-byte aligned; out may alias x.
  */
 GPA_API int gpa_gelu_bf16(const void* x, int64_t n, void* out, void* stream);
+
+/*
+ * Gated residual with the norms around it (the residual adds, LayerScales and
+ * norms of vggt/layers/block.py:85-94 and layer_scale.py:21; the gate of
+ * vggt/heads/camera_head.py), one pass:
+ *   z[r] = x[r] + gate[r / gate_rows] * P(y[r]),   h[r] = N(z[r])
+ * P: post_kind GPA_NORM_NONE (y itself), _LAYER or _RMS with optional
+ * post_weight / post_bias; N: kind likewise with weight / bias (GPA_NORM_NONE:
+ * no h is written).  gate NULL: 1; else [rows / gate_rows, cols], each row
+ * shared by gate_rows consecutive rows.  x, z: x_dtype (the stream); y, h:
+ * y_dtype; an f32 branch needs an f32 stream.  Parameters are all of
+ * param_dtype.  fp32 arithmetic; gate * P(y) is rounded to x_dtype before the
+ * add, N normalises z as stored.  cols % 8 == 0, cols <= 8192; row strides in
+ * elements, multiples of 8; 16-byte aligned pointers.  z may be x's or y's
+ * memory, h too, unless it is z's.  stats: NULL, or [rows, 4] fp32 for the
+ * backward pass.
+ */
+GPA_API int gpa_residual_norm(const void* x, int x_dtype, int64_t x_stride, const void* y, int y_dtype,
+                              int64_t y_stride, const void* gate, int gate_dtype, int64_t gate_rows,
+                              int rows, int cols, int post_kind, const void* post_weight,
+                              const void* post_bias, float post_eps, int kind, const void* weight,
+                              const void* bias, int param_dtype, float eps, void* z, int64_t z_stride,
+                              void* h, int64_t h_stride, float* stats, void* stream);
+
+/*
+ * Its gradients.  dz, dh: gradients of z and h (either may be NULL: zero); z,
+ * y, stats, gate and parameters as in the forward call.  Writes dx [rows, cols]
+ * x_dtype and dy y_dtype, and where not NULL dgate (gate_dtype, gate's shape),
+ * dweight, dbias, dpost_weight, dpost_bias (param_dtype, [cols]); the column
+ * sums run in fp32 in a fixed order.  rows > 0.  workspace: 16-byte aligned,
+ * gpa_residual_norm_backward_workspace_bytes(rows, cols, gate_rows) bytes with
+ * gate_rows = rows when there is no gate; calls that may overlap need their own.
+ */
+GPA_API int64_t gpa_residual_norm_backward_workspace_bytes(int rows, int cols, int64_t gate_rows);
+GPA_API int gpa_residual_norm_backward(
+    const void* dz, int64_t dz_stride, const void* dh, int64_t dh_stride, const void* z, int x_dtype,
+    int64_t z_stride, const void* y, int y_dtype, int64_t y_stride, const float* stats, const void* gate,
+    int gate_dtype, int64_t gate_rows, int rows, int cols, int post_kind, const void* post_weight,
+    const void* post_bias, int kind, const void* weight, int param_dtype, void* dx, int64_t dx_stride,
+    void* dy, int64_t dy_stride, void* dgate, void* dweight, void* dbias, void* dpost_weight,
+    void* dpost_bias, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,12 @@ SIGNATURES = {
                                             _c_i64, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _vp,
                                             _vp, _c_int, _vp, _c_int, _vp, _c_i64, _vp, _c_i64, _vp, _vp,
                                             _vp, _vp, _vp, _vp, _c_i64, _vp]),
+    "gpa_attention_shared_prefix_workspace_bytes": (_c_i64, [_c_int] * 7),
+    "gpa_attention_shared_prefix": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64,
+                                             _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64,
+                                             _c_i64, _c_i64, _vp, _vp] + [_c_int] * 7 + [_c_f32, _c_int, _vp,
+                                             _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp,
+                                             _vp]),
     "gpa_lse_combine": (_c_int, [_c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _vp]),
 }

@@ -1,0 +1,575 @@
+// Attention of a batch of requests over prefix keys that all of them share and
+// over each request's own cached keys (one softmax over both):
+//   s_ij = scale * q_i . k_j + bias_j     (prefix keys; own keys without bias)
+//   o_i  = sum_j softmax_j(s_i) v_j,      lse_i = log2 of the softmax denominator
+//
+// The prefix is read once for all requests: the queries of every request that
+// use one key/value head are rows of the same tile.  The keys are split into
+// chunks, an item is (row tile, key/value head, chunk) of the prefix or of one
+// request's cache, and each writes its unnormalised output, maximum and sum; a
+// second kernel joins the chunks of a row:
+//   m = max m_c, l = sum l_c 2^(m_c - m), o = sum o_c 2^(m_c - m) / l.
+// Scores, statistics and partial outputs are fp32; the probabilities are rounded
+// to bf16 for the product with V (their sum is not).
+//
+// Few rows per tile make this a stream of K and V from HBM: 16 to 64 rows on
+// mma.sync tiles, whose rate suffices there (64 rows need 64 flop per byte, 0.4
+// PFLOP/s at the full HBM rate).  K and V come through a cp.async ring of 64-key
+// tiles, three CTAs per SM (two at head_dim 128).
+#include "common.cuh"
+#include "capi_util.h"
+
+namespace gpa {
+namespace prefix {
+
+constexpr int BN = 64;         // keys per tile
+constexpr int THREADS = 128;
+constexpr int kSlotTiles = 4;  // at least this many tiles per chunk
+
+struct Params {
+  const __nv_bfloat16 *q, *kp, *vp, *ko, *vo;
+  const float* bias;
+  const int32_t *own_len, *q_len;
+  int requests, queries, heads, kv_heads, group, prefix, cache;
+  int64_t q_sr, q_sh, q_sm, kp_sh, kp_sn, vp_sh, vp_sn, ko_sr, ko_sh, ko_sn, vo_sr, vo_sh, vo_sn, bias_sh;
+  float scale_log2;
+  int causal;
+  __nv_bfloat16* o;
+  int64_t o_sr, o_sh, o_sm;
+  float* lse;
+  int64_t lse_sr, lse_sh;
+  // items: row tiles x chunks of the prefix per key head, then of each request's cache
+  int rt1, s1, rt2, s2, chunk;   // chunk in keys
+  int64_t rows;                  // requests * queries * heads
+  float* ws_o;                   // [s1 + s2][rows][D]
+  float2* ws_ml;                 // [s1 + s2][rows]: maximum (log2 units) and sum
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int TILE = BN * D * 2;                    // bytes of a K or V tile
+  static constexpr int STAGE = 2 * TILE + BN * 4;            // K, V, bias
+  static constexpr int SMEM = STAGES * STAGE;
+  static constexpr int CTAS = D == 64 ? 3 : 2;
+  static_assert(SMEM * CTAS <= 227 * 1024 - CTAS * 1024, "shared memory of the resident CTAs");
+  static_assert(4 * 16 * (D + 2) * 4 <= SMEM, "the warps' partial outputs reuse the ring");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+  const int n = in ? 16 : 0;   // zero fill past the end
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte offset of 16-byte chunk c of key row in a tile: rows of D bf16, the
+// chunk's low three bits swapped around by the row, so that eight rows of one
+// chunk column lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t swz(int row, int c) {
+  return row * (D * 2) + (((c & ~7) | ((c ^ row) & 7)) << 4);
+}
+
+// A prefix bias in log2 units.  -inf (or NaN) takes the key out; the type's
+// lowest values stay finite, so keys that all carry them are still weighed.
+__device__ __forceinline__ float bias_log2(float b) {
+  return b > -INFINITY ? fminf(fmaxf(b * 1.4426950408889634f, -3.402823466e38f), 3.402823466e38f) : -INFINITY;
+}
+
+// The rows of a tile: row i of it is query head kh * group + i % group of token
+// (i / group), tokens counted through all requests (prefix) or within one (own).
+struct Row {
+  int r, m, h;
+  bool live;
+};
+template <bool OWN>
+__device__ __forceinline__ Row row_of(const Params& p, int i, int req, int kh) {
+  Row w;
+  const int tok = i / p.group;
+  w.h = kh * p.group + (i - tok * p.group);
+  w.r = OWN ? req : tok / p.queries;
+  w.m = OWN ? tok : tok - w.r * p.queries;
+  w.live = OWN ? tok < p.queries : w.r < p.requests;
+  if (w.live && p.q_len) w.live = w.m < __ldg(p.q_len + w.r);
+  return w;
+}
+
+// One item.  WM warps of 16 rows each; the 4 / WM warps that share the rows
+// split each tile's keys and are joined at the end.
+template <int D, int WM, bool OWN>
+__device__ __forceinline__ void run_item(const Params& p, uint8_t* smem, int kh, int req, int tile, int slot) {
+  using C = Cfg<D>;
+  constexpr int WK = 4 / WM;
+  constexpr int KW = BN / WK;          // keys of a tile per warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wm = warp % WM, wk = warp / WM;
+  const int row0 = tile * (16 * WM) + wm * 16;
+
+  int len = OWN ? p.cache : p.prefix;
+  int qlen = p.queries;
+  if (OWN) {
+    if (p.own_len) len = min(max(__ldg(p.own_len + req), 0), p.cache);
+    if (p.q_len) qlen = min(max(__ldg(p.q_len + req), 0), p.queries);
+  }
+  const int k0 = slot * p.chunk, k1 = min(len, k0 + p.chunk);
+  const int64_t base = (int64_t)(OWN ? p.s1 + slot : slot) * p.rows;
+  auto row_at = [&](const Row& w) { return base + ((int64_t)w.r * p.queries + w.m) * p.heads + w.h; };
+  if (k0 >= k1) {   // nothing here: no output, a sum of zero
+    if (threadIdx.x < 16 * WM) {
+      const Row w = row_of<OWN>(p, tile * (16 * WM) + threadIdx.x, req, kh);
+      if (w.live) p.ws_ml[row_at(w)] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  const Row ra = row_of<OWN>(p, row0 + (lane >> 2), req, kh), rb = row_of<OWN>(p, row0 + (lane >> 2) + 8, req, kh);
+  const int nt = (k1 - k0 + BN - 1) / BN;
+  // keys that a row sees end here (own keys in order: the last query sees them all)
+  const int ea = OWN && p.causal ? len - qlen + ra.m + 1 : k1, eb = OWN && p.causal ? len - qlen + rb.m + 1 : k1;
+
+  const __nv_bfloat16* kbase = OWN ? p.ko + req * p.ko_sr + kh * p.ko_sh : p.kp + kh * p.kp_sh;
+  const __nv_bfloat16* vbase = OWN ? p.vo + req * p.vo_sr + kh * p.vo_sh : p.vp + kh * p.vp_sh;
+  const int64_t ksn = OWN ? p.ko_sn : p.kp_sn, vsn = OWN ? p.vo_sn : p.vp_sn;
+  const float* bias = OWN || !p.bias ? nullptr : p.bias + kh * p.bias_sh;
+  const uint32_t sbase = smem_u32(smem);
+
+  auto issue = [&](int j) {
+    if (j < nt) {
+      const uint32_t st = sbase + (j % C::STAGES) * C::STAGE;
+      constexpr int CPR = D / 8;                       // 16-byte chunks per row
+      const int c = threadIdx.x % CPR;
+#pragma unroll
+      for (int i = 0; i < BN / (THREADS / CPR); ++i) {
+        const int row = threadIdx.x / CPR + i * (THREADS / CPR);
+        const int key = k0 + j * BN + row;
+        const bool in = key < k1;
+        const int64_t kk = in ? key : k0;
+        cp16(st + swz<D>(row, c), kbase + kk * ksn + c * 8, in);
+        cp16(st + C::TILE + swz<D>(row, c), vbase + kk * vsn + c * 8, in);
+      }
+      if (bias && threadIdx.x < BN) {
+        const int key = min(k0 + j * BN + (int)threadIdx.x, k1 - 1);
+        cp4(st + 2 * C::TILE + threadIdx.x * 4, bias + key);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < C::STAGES - 1; ++j) issue(j);
+
+  // Q fragments straight from memory: 16 rows x D of this warp
+  uint32_t qf[D / 16][4];
+  {
+    const __nv_bfloat16* qa = p.q + ra.r * p.q_sr + ra.h * p.q_sh + ra.m * p.q_sm + (lane & 3) * 2;
+    const __nv_bfloat16* qb = p.q + rb.r * p.q_sr + rb.h * p.q_sh + rb.m * p.q_sm + (lane & 3) * 2;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      qf[k][0] = ra.live ? __ldg(reinterpret_cast<const uint32_t*>(qa + k * 16)) : 0u;
+      qf[k][1] = rb.live ? __ldg(reinterpret_cast<const uint32_t*>(qb + k * 16)) : 0u;
+      qf[k][2] = ra.live ? __ldg(reinterpret_cast<const uint32_t*>(qa + k * 16 + 8)) : 0u;
+      qf[k][3] = rb.live ? __ldg(reinterpret_cast<const uint32_t*>(qb + k * 16 + 8)) : 0u;
+    }
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+
+  for (int j = 0; j < nt; ++j) {
+    cp_wait<C::STAGES - 2>();
+    __syncthreads();
+    issue(j + C::STAGES - 1);
+    const int st = (j % C::STAGES) * C::STAGE;
+    const uint32_t sk = sbase + st, sv = sk + C::TILE;
+    float* sb = reinterpret_cast<float*>(smem + st + 2 * C::TILE);
+    const int kt = k0 + j * BN;           // first key of the tile
+    if (bias) {
+      // Keys that the bias takes out count as absent: their K and V may hold
+      // anything, so they are zeroed here by every warp that reads them.
+      bool out = false;
+#pragma unroll
+      for (int i = 0; i < KW; i += 32) out |= (KW >= 32 || lane < KW) && !(sb[wk * KW + (i + lane) % KW] > -INFINITY);
+      unsigned any = __ballot_sync(0xffffffffu, out);
+      if (any) {
+        for (int row = wk * KW; row < wk * KW + KW; ++row)
+          if (!(sb[row] > -INFINITY) && lane < D / 8) {
+            *reinterpret_cast<uint4*>(smem + st + swz<D>(row, lane)) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(smem + st + C::TILE + swz<D>(row, lane)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        __syncwarp();
+      }
+    }
+    float s[KW / 8][4];
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {   // 8 keys x 32 features
+        uint32_t b[4];
+        ldsm4(sk + swz<D>(wk * KW + n * 8 + (lane & 7), k * 4 + (lane >> 3)), b);
+        mma(s[n], qf[2 * k], b[0], b[1]);
+        mma(s[n], qf[2 * k + 1], b[2], b[3]);
+      }
+    }
+    // scale, bias, mask
+    const bool edge = kt + BN > k1 || (OWN && p.causal && kt + BN > len - qlen + 1);
+    float xa = -INFINITY, xb = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n) {
+      const int col = wk * KW + n * 8 + (lane & 3) * 2;
+      float b0 = 0.f, b1 = 0.f;
+      if (bias) {
+        const float2 bb = *reinterpret_cast<const float2*>(sb + col);
+        b0 = bias_log2(bb.x);
+        b1 = bias_log2(bb.y);
+      }
+      s[n][0] = fmaf(s[n][0], p.scale_log2, b0);
+      s[n][1] = fmaf(s[n][1], p.scale_log2, b1);
+      s[n][2] = fmaf(s[n][2], p.scale_log2, b0);
+      s[n][3] = fmaf(s[n][3], p.scale_log2, b1);
+      if (edge) {
+        const int key = kt + col;
+        const int ca = min(ea, k1), cb = min(eb, k1);
+        if (key >= ca) s[n][0] = -INFINITY;
+        if (key + 1 >= ca) s[n][1] = -INFINITY;
+        if (key >= cb) s[n][2] = -INFINITY;
+        if (key + 1 >= cb) s[n][3] = -INFINITY;
+      }
+      xa = fmaxf(xa, fmaxf(s[n][0], s[n][1]));
+      xb = fmaxf(xb, fmaxf(s[n][2], s[n][3]));
+    }
+    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
+    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
+    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
+    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
+    if (xa > ma || xb > mb) {   // quads move on their own
+      const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
+      const float fa = na > ma ? fast_exp2(ma - na) : 1.f, fb = nb > mb ? fast_exp2(mb - nb) : 1.f;
+      ma = na;
+      mb = nb;
+      la *= fa;
+      lb *= fb;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= fa;
+        o[i][1] *= fa;
+        o[i][2] *= fb;
+        o[i][3] *= fb;
+      }
+    }
+    __syncwarp();
+    const float sa = ma > -INFINITY ? ma : 0.f, sbm = mb > -INFINITY ? mb : 0.f;
+#pragma unroll
+    for (int k = 0; k < KW / 16; ++k) {
+      uint32_t pf[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float* x = s[2 * k + u];
+        const float e0 = fast_exp2(x[0] - sa), e1 = fast_exp2(x[1] - sa);
+        const float e2 = fast_exp2(x[2] - sbm), e3 = fast_exp2(x[3] - sbm);
+        la += e0 + e1;
+        lb += e2 + e3;
+        pf[2 * u] = pack_bf16x2(e0, e1);
+        pf[2 * u + 1] = pack_bf16x2(e2, e3);
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {   // 16 keys x 16 features of V
+        uint32_t b[4];
+        ldsm4t(sv + swz<D>(wk * KW + k * 16 + (lane & 15), d * 2 + (lane >> 4)), b);
+        mma(o[2 * d], pf, b[0], b[1]);
+        mma(o[2 * d + 1], pf, b[2], b[3]);
+      }
+    }
+  }
+  la += __shfl_xor_sync(0xffffffffu, la, 1);
+  la += __shfl_xor_sync(0xffffffffu, la, 2);
+  lb += __shfl_xor_sync(0xffffffffu, lb, 1);
+  lb += __shfl_xor_sync(0xffffffffu, lb, 2);
+
+  if constexpr (WK == 1) {
+    if (ra.live) {
+      const int64_t at = row_at(ra);
+      if ((lane & 3) == 0) p.ws_ml[at] = make_float2(ma, la);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(p.ws_o + at * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][0], o[i][1]);
+    }
+    if (rb.live) {
+      const int64_t at = row_at(rb);
+      if ((lane & 3) == 0) p.ws_ml[at] = make_float2(mb, lb);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(p.ws_o + at * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2], o[i][3]);
+    }
+  } else {
+    // join the WK warps of a row through the ring's memory
+    cp_wait<0>();
+    __syncthreads();
+    float* po = reinterpret_cast<float*>(smem);                 // [4 warps][16 rows][D]
+    float2* pm = reinterpret_cast<float2*>(po + 4 * 16 * D);     // [4 warps][16 rows]
+    const int a = lane >> 2;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      *reinterpret_cast<float2*>(po + (warp * 16 + a) * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][0], o[i][1]);
+      *reinterpret_cast<float2*>(po + (warp * 16 + a + 8) * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2], o[i][3]);
+    }
+    if ((lane & 3) == 0) {
+      pm[warp * 16 + a] = make_float2(ma, la);
+      pm[warp * 16 + a + 8] = make_float2(mb, lb);
+    }
+    __syncthreads();
+    // a warp takes rows in turn, its lanes the features
+    for (int i = warp; i < 16 * WM; i += 4) {
+      const Row w = row_of<OWN>(p, tile * (16 * WM) + i, req, kh);
+      if (!w.live) continue;
+      const int q0 = (i >> 4) * 16 + (i & 15);    // this row in the first of its warps
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < WK; ++c) m = fmaxf(m, pm[c * WM * 16 + q0].x);
+      float v[D / 32];
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) v[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < WK; ++c) {
+        const float2 ml = pm[c * WM * 16 + q0];
+        const float f = ml.x > -INFINITY ? fast_exp2(ml.x - m) : 0.f;
+        l += ml.y * f;
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) v[u] = fmaf(f, po[(c * WM * 16 + q0) * D + u * 32 + lane], v[u]);
+      }
+      const int64_t at = row_at(w);
+      if (lane == 0) p.ws_ml[at] = make_float2(m, l);
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) p.ws_o[at * D + u * 32 + lane] = v[u];
+    }
+  }
+}
+
+template <int D, int WM1, int WM2>
+__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  // items of the prefix: row tile fastest (its CTAs share the keys in L2)
+  int64_t it = blockIdx.x;
+  const int64_t n1 = (int64_t)p.kv_heads * p.s1 * p.rt1;
+  if (it < n1) {
+    const int t = (int)(it % p.rt1);
+    it /= p.rt1;
+    run_item<D, WM1, false>(p, smem, (int)(it / p.s1), 0, t, (int)(it % p.s1));
+    return;
+  }
+  it -= n1;
+  const int t = (int)(it % p.rt2);
+  it /= p.rt2;
+  const int s = (int)(it % p.s2);
+  it /= p.s2;
+  run_item<D, WM2, true>(p, smem, (int)(it % p.kv_heads), (int)(it / p.kv_heads), t, s);
+}
+
+// Joins a row's chunks: one warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= p.rows) return;
+  const int h = (int)(row % p.heads);
+  const int64_t tok = row / p.heads;
+  const int m = (int)(tok % p.queries), r = (int)(tok / p.queries);
+  if (p.q_len && m >= __ldg(p.q_len + r)) return;
+  const int slots = p.s1 + p.s2;
+  float mx = -INFINITY;
+  for (int s = lane; s < slots; s += 32) mx = fmaxf(mx, p.ws_ml[(int64_t)s * p.rows + row].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  float l = 0.f, v[D / 32];
+#pragma unroll
+  for (int u = 0; u < D / 32; ++u) v[u] = 0.f;
+  for (int s0 = 0; s0 < slots; s0 += 32) {
+    float f = 0.f;
+    if (s0 + lane < slots) {
+      const float2 ml = p.ws_ml[(int64_t)(s0 + lane) * p.rows + row];
+      f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
+      l = fmaf(ml.y, f, l);
+    }
+    const int n = min(32, slots - s0);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      if (w > 0.f) {   // an empty chunk wrote no output
+        const float* o = p.ws_o + ((int64_t)(s0 + i) * p.rows + row) * D + lane * (D / 32);
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) v[u] = fmaf(w, o[u], v[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
+  __nv_bfloat16* orow = p.o + r * p.o_sr + h * p.o_sh + m * p.o_sm + lane * (D / 32);
+  if constexpr (D == 64) {
+    *reinterpret_cast<uint32_t*>(orow) = pack_bf16x2(v[0] * inv, v[1] * inv);
+  } else {
+    *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+  }
+  if (p.lse && lane == 0) p.lse[r * p.lse_sr + h * p.lse_sh + m] = l == 0.f ? -INFINITY : mx + log2f(l);
+}
+
+// How a call is cut into items.
+struct Plan {
+  int wm1, rt1, s1, wm2, rt2, s2, chunk;
+  int64_t items, rows;
+};
+
+static int warps_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+static Plan make_plan(int requests, int queries, int heads, int kv_heads, int head_dim, int prefix, int cache) {
+  Plan p;
+  const int group = heads / kv_heads;
+  const int64_t r1 = (int64_t)requests * queries * group, r2 = (int64_t)queries * group;
+  p.rows = r1 * kv_heads;
+  p.wm1 = warps_for(r1);
+  p.wm2 = warps_for(r2);
+  p.rt1 = (int)((r1 + p.wm1 * 16 - 1) / (p.wm1 * 16));
+  p.rt2 = (int)((r2 + p.wm2 * 16 - 1) / (p.wm2 * 16));
+  const int64_t t1 = (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
+  const int64_t units = kv_heads * (p.rt1 * t1 + (int64_t)requests * p.rt2 * t2);
+  // two items per resident CTA: short enough to even out requests of unequal
+  // lengths, long enough that the partial outputs are a small share
+  const int64_t want = 148ll * (head_dim == 64 ? 3 : 2) * 2;
+  const int64_t per = std::max<int64_t>((units + want - 1) / want, kSlotTiles);
+  p.chunk = (int)std::min<int64_t>(per, 1 << 24) * BN;
+  p.s1 = (int)((t1 + per - 1) / per);
+  p.s2 = (int)((t2 + per - 1) / per);
+  p.items = kv_heads * ((int64_t)p.rt1 * p.s1 + (int64_t)requests * p.rt2 * p.s2);
+  return p;
+}
+
+template <int D, int WM1, int WM2>
+static int launch_rows(const Params& p, int64_t items, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, WM1, WM2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
+  rows_kernel<D, WM1, WM2><<<(unsigned)items, THREADS, Cfg<D>::SMEM, st>>>(p);
+  return check_launch("gpa_attention_shared_prefix");
+}
+
+template <int D>
+static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
+  int rc = GPA_OK;
+  if (plan.items > 0) {
+    switch (plan.wm1 * 8 + plan.wm2) {   // wm2 <= wm1: own rows are part of the prefix's
+      case 1 * 8 + 1: rc = launch_rows<D, 1, 1>(p, plan.items, st); break;
+      case 2 * 8 + 1: rc = launch_rows<D, 2, 1>(p, plan.items, st); break;
+      case 2 * 8 + 2: rc = launch_rows<D, 2, 2>(p, plan.items, st); break;
+      case 4 * 8 + 1: rc = launch_rows<D, 4, 1>(p, plan.items, st); break;
+      case 4 * 8 + 2: rc = launch_rows<D, 4, 2>(p, plan.items, st); break;
+      default: rc = launch_rows<D, 4, 4>(p, plan.items, st); break;
+    }
+  }
+  if (rc) return rc;
+  join_kernel<D><<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>(p);
+  return check_launch("gpa_attention_shared_prefix");
+}
+
+static int check_sizes(const char* what, int requests, int queries, int heads, int kv_heads, int head_dim, int prefix,
+                       int cache) {
+  if (requests < 0 || queries < 0 || heads <= 0 || kv_heads <= 0 || prefix < 0 || cache < 0 || heads % kv_heads)
+    return fail(GPA_ERR_INVALID, "%s: bad sizes (heads must be a multiple of kv_heads)", what);
+  if (head_dim != 64 && head_dim != 128) return fail(GPA_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", what);
+  if ((double)requests * queries * heads >= 2147483648.0)
+    return fail(GPA_ERR_UNSUPPORTED, "%s: 2^31 or more query rows", what);
+  if (prefix > (1 << 30) || cache > (1 << 30)) return fail(GPA_ERR_UNSUPPORTED, "%s: more than 2^30 keys", what);
+  return GPA_OK;
+}
+
+}  // namespace prefix
+}  // namespace gpa
+
+using namespace gpa;
+
+extern "C" int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int queries, int heads, int kv_heads,
+                                                               int head_dim, int prefix, int cache) {
+  if (prefix::check_sizes("gpa_attention_shared_prefix_workspace_bytes", requests, queries, heads, kv_heads, head_dim,
+                          prefix, cache))
+    return -1;
+  if (requests == 0 || queries == 0) return 0;
+  const prefix::Plan p = prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache);
+  return (int64_t)(p.s1 + p.s2) * p.rows * (head_dim + 2) * 4;
+}
+
+extern "C" int gpa_attention_shared_prefix(
+    const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, const void* k_prefix, int64_t kp_sh, int64_t kp_sn,
+    const void* v_prefix, int64_t vp_sh, int64_t vp_sn, const float* bias, int64_t bias_sh, const void* k_own,
+    int64_t ko_sr, int64_t ko_sh, int64_t ko_sn, const void* v_own, int64_t vo_sr, int64_t vo_sh, int64_t vo_sn,
+    const int32_t* own_len, const int32_t* q_len, int requests, int queries, int heads, int kv_heads, int head_dim,
+    int prefix_len, int cache_len, float sm_scale, int causal, void* o, int64_t o_sr, int64_t o_sh, int64_t o_sm,
+    float* lse, int64_t lse_sr, int64_t lse_sh, void* workspace, int64_t workspace_bytes, int* status, void* stream) {
+  const char* what = "gpa_attention_shared_prefix";
+  int rc = prefix::check_sizes(what, requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len);
+  if (rc) return rc;
+  if (requests == 0 || queries == 0) return ok();
+  if (!q || !o || (prefix_len && (!k_prefix || !v_prefix)) || (cache_len && (!k_own || !v_own)))
+    return fail(GPA_ERR_INVALID, "%s: null pointer", what);
+  if (!aligned16(q) || !aligned16(o) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_own) ||
+      !aligned16(v_own))
+    return fail(GPA_ERR_INVALID, "%s: q, keys, values and o must be 16-byte aligned", what);
+  if ((q_sr | q_sh | q_sm | kp_sh | kp_sn | vp_sh | vp_sn | ko_sr | ko_sh | ko_sn | vo_sr | vo_sh | vo_sn | o_sr |
+       o_sh | o_sm) & 7)
+    return fail(GPA_ERR_INVALID, "%s: strides must be multiples of 8", what);
+  if (!prefix_len) bias = nullptr;
+  const prefix::Plan plan = prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len);
+  if (plan.items >= (1ll << 31)) return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
+  const int64_t slots = plan.s1 + plan.s2;
+  if (slots && (!workspace || !aligned16(workspace) || workspace_bytes < slots * plan.rows * (head_dim + 2) * 4))
+    return fail(GPA_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
+  prefix::Params p;
+  p.q = (const __nv_bfloat16*)q;
+  p.kp = (const __nv_bfloat16*)k_prefix;
+  p.vp = (const __nv_bfloat16*)v_prefix;
+  p.ko = (const __nv_bfloat16*)k_own;
+  p.vo = (const __nv_bfloat16*)v_own;
+  p.bias = bias;
+  p.own_len = own_len;
+  p.q_len = q_len;
+  p.requests = requests;
+  p.queries = queries;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = heads / kv_heads;
+  p.prefix = prefix_len;
+  p.cache = cache_len;
+  p.q_sr = q_sr; p.q_sh = q_sh; p.q_sm = q_sm;
+  p.kp_sh = kp_sh; p.kp_sn = kp_sn; p.vp_sh = vp_sh; p.vp_sn = vp_sn;
+  p.ko_sr = ko_sr; p.ko_sh = ko_sh; p.ko_sn = ko_sn;
+  p.vo_sr = vo_sr; p.vo_sh = vo_sh; p.vo_sn = vo_sn;
+  p.bias_sh = bias_sh;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.causal = causal;
+  p.o = (__nv_bfloat16*)o;
+  p.o_sr = o_sr; p.o_sh = o_sh; p.o_sm = o_sm;
+  p.lse = lse;
+  p.lse_sr = lse_sr; p.lse_sh = lse_sh;
+  p.rt1 = plan.rt1; p.s1 = plan.s1; p.rt2 = plan.rt2; p.s2 = plan.s2; p.chunk = plan.chunk;
+  p.rows = plan.rows;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = reinterpret_cast<float2*>(p.ws_o + slots * plan.rows * head_dim);
+  cudaStream_t st = (cudaStream_t)stream;
+  return head_dim == 64 ? prefix::launch<64>(p, plan, st) : prefix::launch<128>(p, plan, st);
+}

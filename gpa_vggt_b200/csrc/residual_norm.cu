@@ -9,12 +9,12 @@
 // reads dz, dh, z, y and writes dx, dy.  Everything of a row stays in registers
 // between its load and its store, and all arithmetic is fp32.
 //
-// Roundings: z is kept in the stream's type, the branch term gate * P(y) is
-// rounded to that type before the add, and N normalises z as kept.  For a bf16
-// stream these are the roundings of residual_scale followed by layernorm
-// (norm.cu), so a block that changes from the two kernels to this one keeps its
-// results bit for bit (up to 2,048 columns, where the sums also run in the same
-// order).
+// Roundings: z is kept in the stream's type and N normalises z as kept; without
+// a norm of the branch, gate * y is rounded to the stream's type before the add.
+// For a bf16 stream these are the roundings of residual_scale followed by
+// layernorm (norm.cu), so a block that changes from the two kernels to this one
+// keeps its results bit for bit (up to 2,048 columns, where the sums also run in
+// the same order).
 #include "common.cuh"
 #include "capi_util.h"
 
@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(256) fwd_kernel(const FwdParams p) {
       float x8[8];
       xv[u].get(x8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[u][i] = round_to<TX>(__fadd_rn(x8[i], round_to<TX>(v[i])));
+      for (int i = 0; i < 8; ++i)
+        z[u][i] = round_to<TX>(__fadd_rn(x8[i], p.post_kind == kNone ? round_to<TX>(v[i]) : v[i]));
       store8(zr + c, z[u]);
     }
 #pragma unroll

@@ -402,6 +402,107 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
     return (out, lse) if return_lse else out
 
 
+def _kernel_strides(t: torch.Tensor):
+    """Strides of all dims but the last, 0 where a dim has at most one entry."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+
+
+def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out):
+    what = "attention_shared_prefix"
+    if q.dim() != 4 or k_prefix.dim() != 3 or k_own.dim() != 4:
+        raise ValueError(f"{what}: q [R,H,M,D], k_prefix [Hk,P,D] and k_own [R,Hk,N,D] required")
+    R, H, M, D = q.shape
+    Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]
+    if (tuple(v_prefix.shape) != (Hk, P, D) or tuple(k_prefix.shape) != (Hk, P, D)
+            or tuple(k_own.shape) != (R, Hk, N, D) or tuple(v_own.shape) != (R, Hk, N, D)):
+        raise ValueError(f"{what}: keys and values do not fit q [R,H,M,D]: [Hk,P,D] and [R,Hk,N,D] required")
+    if any(t.dtype != BF16 for t in (q, k_prefix, v_prefix, k_own, v_own)):
+        raise TypeError(f"{what}: q, keys and values must be bf16")
+    if D not in (64, 128):
+        raise ValueError(f"{what}: head dim 64 or 128 required")
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{what}: the query heads must be a multiple of the key heads")
+    for t in (own_len, q_len):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"{what}: own_len and q_len must be int32")
+        if t is not None and tuple(t.shape) != (R,):
+            raise ValueError(f"{what}: own_len and q_len must be [R]")
+    if bias is not None:
+        if not bias.is_floating_point():
+            raise TypeError(f"{what}: bias must be a floating type")
+        if bias.dim() not in (1, 2) or bias.shape[-1] != P or (bias.dim() == 2 and bias.shape[0] not in (1, Hk)):
+            raise ValueError(f"{what}: bias must be [P], [1,P] or [Hk,P]")
+    if out is not None and (out.dtype != BF16 or tuple(out.shape) != (R, H, M, D)
+                            or (out.numel() and not _tma_ok(out))):
+        raise ValueError(f"{what}: out must be a bf16 [R,H,M,D] view, innermost contiguous, 16-byte aligned rows")
+    if lse_out is not None and (lse_out.dtype != F32 or tuple(lse_out.shape) != (R, H, M)
+                                or (M > 1 and lse_out.stride(-1) != 1)):
+        raise ValueError(f"{what}: lse_out must be an fp32 [R,H,M] view with row stride 1")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k_prefix, v_prefix, k_own, v_own, bias)):
+        raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
+    return _device_of(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, what=what)
+
+
+def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
+                            k_own: torch.Tensor, v_own: torch.Tensor, sm_scale: float,
+                            own_len: Optional[torch.Tensor] = None, q_len: Optional[torch.Tensor] = None,
+                            bias: Optional[torch.Tensor] = None, causal: bool = False,
+                            return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                            lse_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+    """Attention of R requests over prefix keys that all of them share and over
+    each request's own cached keys, one softmax over both: the merged K/V of a
+    mapped scene (bias = its log counts) as the prefix of every stream that is
+    localised in it, say.  The prefix is read once for all requests.
+
+    q [R,H,M,D], k_prefix / v_prefix [Hk,P,D], k_own / v_own [R,Hk,N,D], bf16,
+    any strides with the innermost dim contiguous, D 64 or 128, H a multiple of
+    Hk (H/Hk query heads in a row share a key head).  own_len, q_len: int32 [R]
+    on the device (clamped to [0,N] and [0,M]), or None for all N and M; cache
+    rows past own_len may hold anything.  bias: [P], [1,P] or [Hk,P], natural-log
+    domain; -inf (or NaN) takes a key out, whatever its K and V hold.  causal:
+    query i sees own keys j <= own_len - q_len + i, and every prefix key.
+
+    Returns out [R,H,M,D] bf16, and with return_lse (or lse_out) the log2 row
+    sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len
+    are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
+    -inf.  Nothing is read back to the host, so calls can be captured; no
+    gradients."""
+    device = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out)
+    R, H, M, D = q.shape
+    Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]
+    if out is None:
+        out = (torch.empty if q_len is None else torch.zeros)(R, H, M, D, device=device, dtype=BF16)
+    if lse_out is None and return_lse:
+        lse_out = (torch.empty(R, H, M, device=device, dtype=F32) if q_len is None
+                   else torch.full((R, H, M), -float("inf"), device=device, dtype=F32))
+    if R * M == 0:
+        return (out, lse_out) if lse_out is not None else out
+    q, k_prefix, v_prefix, k_own, v_own = (t if _tma_ok(t) else t.clone(memory_format=torch.contiguous_format)
+                                           for t in (q, k_prefix, v_prefix, k_own, v_own))
+    bias_sh = 0
+    if bias is not None:
+        bias = bias.detach().to(F32)
+        if P > 1 and bias.stride(-1) != 1:
+            bias = bias.contiguous()
+        if bias.dim() == 2 and bias.shape[0] > 1:
+            bias_sh = bias.stride(0)
+    own_len, q_len = (None if t is None else t.contiguous() for t in (own_len, q_len))
+    size = _lib.load().gpa_attention_shared_prefix_workspace_bytes(R, M, H, Hk, D, P, N)
+    ws = torch.empty(max(size, 16), device=device, dtype=torch.uint8)
+    status, own = _status_word(status, device)
+    ls = (0, 0) if lse_out is None else lse_out.stride()[:2]
+    with _on(device):
+        call("gpa_attention_shared_prefix", ptr(q), *_kernel_strides(q), ptr(k_prefix), *_kernel_strides(k_prefix),
+             ptr(v_prefix), *_kernel_strides(v_prefix), ptr(bias), bias_sh, ptr(k_own), *_kernel_strides(k_own),
+             ptr(v_own), *_kernel_strides(v_own), ptr(own_len), ptr(q_len), R, M, H, Hk, D, P, N, float(sm_scale),
+             int(bool(causal)), ptr(out), *_kernel_strides(out), ptr(lse_out), *ls, ptr(ws), size, ptr(status),
+             stream_of(q))
+    if own:
+        _check_status(status, "gpa_attention_shared_prefix")
+    return (out, lse_out) if lse_out is not None else out
+
+
 def frame_pool(k: torch.Tensor, v: torch.Tensor, num_frames: int, ph: int, pw: int,
                num_special: int, kp: int):
     """Pooled k, v [H, S*npool, 64] bf16 and pool_size [H, S*npool] fp32 from

@@ -393,8 +393,8 @@ GPA_API int gpa_gelu_bf16(const void* x, int64_t n, void* out, void* stream);
  * no h is written).  gate NULL: 1; else [rows / gate_rows, cols], each row
  * shared by gate_rows consecutive rows.  x, z: x_dtype (the stream); y, h:
  * y_dtype; an f32 branch needs an f32 stream.  Parameters are all of
- * param_dtype.  fp32 arithmetic; gate * P(y) is rounded to x_dtype before the
- * add, N normalises z as stored.  cols % 8 == 0, cols <= 8192; row strides in
+ * param_dtype.  fp32 arithmetic; gate * y without a post norm is rounded to
+ * x_dtype before the add, N normalises z as stored.  cols % 8 == 0, cols <= 8192; row strides in
  * elements, multiples of 8; 16-byte aligned pointers.  z may be x's or y's
  * memory, h too, unless it is z's.  stats: NULL, or [rows, 4] fp32 for the
  * backward pass.
@@ -423,6 +423,39 @@ GPA_API int gpa_residual_norm_backward(
     const void* post_bias, int kind, const void* weight, int param_dtype, void* dx, int64_t dx_stride,
     void* dy, int64_t dy_stride, void* dgate, void* dweight, void* dbias, void* dpost_weight,
     void* dpost_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention of a batch of requests over prefix keys that all share and over
+ * each request's own cached keys, one softmax over both (beside
+ * gpa_attention_keybias, merging/fused_attention.py:130-180, which has one key
+ * set per batch element):
+ *   s_ij = q_i . k_j * sm_scale + bias[kv_head, j]   prefix keys j < prefix
+ *   s_ij = q_i . k_j * sm_scale                      own keys j < own_len[r]
+ *   o_i = sum_j softmax_j(s_i) v_j,  lse_i = log2 of the denominator (as there)
+ * q, o: [requests, heads, queries, head_dim]; k_prefix, v_prefix: [kv_heads,
+ * prefix, head_dim]; k_own, v_own: [requests, kv_heads, cache, head_dim]; bf16,
+ * each with its element strides (multiples of 8, innermost contiguous, 16-byte
+ * aligned).  heads % kv_heads == 0: heads/kv_heads query heads in a row share
+ * a key head.  head_dim 64 or 128.  bias: fp32 rows at bias + kv_head*bias_sh,
+ * or NULL; -inf (or NaN) takes the key out, whatever its K and V hold.
+ * own_len, q_len: device int32 [requests], or NULL for cache and queries;
+ * read by the kernels, clamped to [0, cache] and [0, queries].  Cache rows past
+ * own_len may hold anything.  Query rows past q_len are neither computed nor
+ * written.  causal: query i of a request sees its own keys j <= own_len - q_len
+ * + i (the last query sees all); the prefix is seen by every query.  A query
+ * without keys gives 0 and lse -inf.  lse: fp32, rows contiguous, or NULL.
+ * workspace: 16-byte aligned, _workspace_bytes() (-1: bad sizes); calls that may
+ * overlap need their own.
+ */
+GPA_API int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int queries, int heads, int kv_heads,
+                                                            int head_dim, int prefix, int cache);
+GPA_API int gpa_attention_shared_prefix(
+    const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, const void* k_prefix, int64_t kp_sh, int64_t kp_sn,
+    const void* v_prefix, int64_t vp_sh, int64_t vp_sn, const float* bias, int64_t bias_sh, const void* k_own,
+    int64_t ko_sr, int64_t ko_sh, int64_t ko_sn, const void* v_own, int64_t vo_sr, int64_t vo_sh, int64_t vo_sn,
+    const int32_t* own_len, const int32_t* q_len, int requests, int queries, int heads, int kv_heads, int head_dim,
+    int prefix, int cache, float sm_scale, int causal, void* o, int64_t o_sr, int64_t o_sh, int64_t o_sm,
+    float* lse, int64_t lse_sr, int64_t lse_sh, void* workspace, int64_t workspace_bytes, int* status, void* stream);
 
 #ifdef __cplusplus
 }

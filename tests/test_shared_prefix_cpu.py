@@ -1,0 +1,92 @@
+"""attention_shared_prefix refuses what it does not compute before anything is
+launched (no GPU needed: shapes and types are checked before the device)."""
+import ctypes
+
+import pytest
+import torch
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from gpa_vggt_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def _args(R=2, H=4, M=3, D=64, Hk=2, P=5, N=7, dtype=BF16):
+    def z(*s):
+        return torch.zeros(*s, dtype=dtype)
+    return [z(R, H, M, D), z(Hk, P, D), z(Hk, P, D), z(R, Hk, N, D), z(R, Hk, N, D), 0.125]
+
+
+@pytest.mark.parametrize("error,change,kw", [
+    (TypeError, dict(dtype=F32), {}),
+    (ValueError, dict(D=96), {}),
+    (ValueError, dict(H=3), {}),                                          # heads not a multiple of the key heads
+    (ValueError, {}, dict(own_len=torch.zeros(3, dtype=torch.int32))),
+    (TypeError, {}, dict(own_len=torch.zeros(2, dtype=torch.int64))),
+    (TypeError, {}, dict(q_len=torch.zeros(2))),
+    (ValueError, {}, dict(bias=torch.zeros(4))),
+    (ValueError, {}, dict(bias=torch.zeros(4, 5))),                       # one row per query head
+    (TypeError, {}, dict(bias=torch.zeros(5, dtype=torch.int32))),
+    (ValueError, {}, dict(out=torch.zeros(2, 4, 3, 64))),                 # not bf16
+    (ValueError, {}, dict(out=torch.zeros(2, 4, 4, 64, dtype=BF16))),
+    (ValueError, {}, dict(out=torch.zeros(2, 4, 3, 68, dtype=BF16)[..., :64])),   # rows not 16-byte aligned
+    (ValueError, {}, dict(lse_out=torch.zeros(2, 4, 3, dtype=BF16))),
+    (ValueError, {}, dict(lse_out=torch.zeros(2, 3, 4).transpose(1, 2))),
+    (ValueError, {}, {}),                                                 # all well, but on the CPU
+])
+def test_refusals(error, change, kw):
+    from gpa_vggt_b200 import kernels
+    with pytest.raises(error, match="attention_shared_prefix"):
+        kernels.attention_shared_prefix(*_args(**change), **kw)
+
+
+@pytest.mark.parametrize("i,shape", [(0, (2, 4, 64)), (1, (2, 6, 64)), (2, (2, 5, 128)), (3, (3, 2, 7, 64)),
+                                     (4, (2, 2, 8, 64)), (1, (1, 2, 5, 64))])
+def test_shapes_that_do_not_fit(i, shape):
+    from gpa_vggt_b200 import kernels
+    args = _args()
+    args[i] = torch.zeros(*shape, dtype=BF16)
+    with pytest.raises(ValueError, match="attention_shared_prefix"):
+        kernels.attention_shared_prefix(*args)
+
+
+def test_gradients_are_refused():
+    from gpa_vggt_b200 import kernels
+    args = _args()
+    args[1].requires_grad_(True)
+    with pytest.raises(ValueError, match="no gradients"):
+        kernels.attention_shared_prefix(*args)
+
+
+def test_c_entry_refusals(lib):
+    ok, odd = ctypes.c_void_p(256), ctypes.c_void_p(264)
+
+    def run(q=ok, kp=ok, ko=ok, o=ok, R=2, M=3, H=4, Hk=2, D=64, P=5, N=7, stride=64, ws=ok, n=1 << 20):
+        return lib.gpa_attention_shared_prefix(q, stride, 64, 64, kp, 64, 64, ok, 64, 64, None, 0, ko, 64, 64, 64,
+                                               ok, 64, 64, 64, None, None, R, M, H, Hk, D, P, N, 0.125, 0, o, 64,
+                                               64, 64, None, 0, 0, ws, n, None, None)
+    assert run(R=0) == 0 and run(M=0) == 0                     # nothing to do
+    assert run(R=-1) == 1 and run(H=3) == 1 and run(Hk=0) == 1 and run(P=-1) == 1 and run(N=-2) == 1
+    assert run(D=32) == 3 and b"head_dim" in lib.gpa_last_error()
+    assert run(R=1 << 20, M=1 << 12) == 3                      # 2^31 query rows
+    assert run(P=(1 << 30) + 1) == 3
+    assert run(q=None) == 1 and run(kp=None) == 1 and run(ko=None) == 1 and run(o=None) == 1
+    assert run(q=odd) == 1 and run(kp=odd) == 1 and run(o=odd) == 1
+    assert run(stride=60) == 1 and b"multiples of 8" in lib.gpa_last_error()
+    assert run(ws=None) == 1 and run(ws=odd) == 1 and run(n=64) == 1 and b"workspace" in lib.gpa_last_error()
+
+
+def test_workspace_size(lib):
+    size = lib.gpa_attention_shared_prefix_workspace_bytes
+    assert size(2, 3, 4, 3, 64, 5, 7) == -1 and size(2, 3, 4, 2, 96, 5, 7) == -1
+    assert size(0, 3, 4, 2, 64, 5, 7) == 0 and size(2, 3, 4, 2, 64, 0, 0) == 0
+    for R, M, H, Hk, D, P, N in [(1, 1, 1, 1, 64, 1, 0), (64, 1, 16, 16, 64, 66845, 1374), (4, 1374, 16, 16, 64, 16711, 1374),
+                                 (5, 1, 16, 16, 64, 219840, 2748), (7, 45, 16, 2, 128, 5001, 777)]:
+        n = size(R, M, H, Hk, D, P, N)
+        row = R * M * H * (D + 2) * 4
+        assert n % row == 0 and n <= 600 * row                 # a partial output per chunk, at most hundreds of chunks
+        assert n < 1 << 30

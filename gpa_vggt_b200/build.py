@@ -24,7 +24,8 @@ OBJ = PKG / "_build"
 HEADER = ROOT / "include" / "gpa_b200.h"
 
 SOURCES = ["merge.cu", "sim_argmax.cu", "attention.cu", "frame.cu", "norm.cu", "dpt.cu", "proj.cu",
-           "exchange.cu", "residual_norm.cu", "prefix_attention.cu"]
+           "exchange.cu", "residual_norm.cu", "prefix_attention.cu",
+           "prefix_attention_tc.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

@@ -16,8 +16,7 @@
 // mma.sync tiles, whose rate suffices there (64 rows need 64 flop per byte, 0.4
 // PFLOP/s at the full HBM rate).  K and V come through a cp.async ring of 64-key
 // tiles, three CTAs per SM (two at head_dim 128).
-#include "common.cuh"
-#include "capi_util.h"
+#include "prefix_attention.cuh"
 
 namespace gpa {
 namespace prefix {
@@ -25,25 +24,6 @@ namespace prefix {
 constexpr int BN = 64;         // keys per tile
 constexpr int THREADS = 128;
 constexpr int kSlotTiles = 4;  // at least this many tiles per chunk
-
-struct Params {
-  const __nv_bfloat16 *q, *kp, *vp, *ko, *vo;
-  const float* bias;
-  const int32_t *own_len, *q_len;
-  int requests, queries, heads, kv_heads, group, prefix, cache;
-  int64_t q_sr, q_sh, q_sm, kp_sh, kp_sn, vp_sh, vp_sn, ko_sr, ko_sh, ko_sn, vo_sr, vo_sh, vo_sn, bias_sh;
-  float scale_log2;
-  int causal;
-  __nv_bfloat16* o;
-  int64_t o_sr, o_sh, o_sm;
-  float* lse;
-  int64_t lse_sr, lse_sh;
-  // items: row tiles x chunks of the prefix per key head, then of each request's cache
-  int rt1, s1, rt2, s2, chunk;   // chunk in keys
-  int64_t rows;                  // requests * queries * heads
-  float* ws_o;                   // [s1 + s2][rows][D]
-  float2* ws_ml;                 // [s1 + s2][rows]: maximum (log2 units) and sum
-};
 
 template <int D>
 struct Cfg {
@@ -96,12 +76,7 @@ __device__ __forceinline__ float bias_log2(float b) {
   return b > -INFINITY ? fminf(fmaxf(b * 1.4426950408889634f, -3.402823466e38f), 3.402823466e38f) : -INFINITY;
 }
 
-// The rows of a tile: row i of it is query head kh * group + i % group of token
-// (i / group), tokens counted through all requests (prefix) or within one (own).
-struct Row {
-  int r, m, h;
-  bool live;
-};
+// Tokens are counted through all requests (prefix) or within one (own).
 template <bool OWN>
 __device__ __forceinline__ Row row_of(const Params& p, int i, int req, int kh) {
   Row w;
@@ -125,15 +100,11 @@ __device__ __forceinline__ void run_item(const Params& p, uint8_t* smem, int kh,
   const int wm = warp % WM, wk = warp / WM;
   const int row0 = tile * (16 * WM) + wm * 16;
 
-  int len = OWN ? p.cache : p.prefix;
-  int qlen = p.queries;
-  if (OWN) {
-    if (p.own_len) len = min(max(__ldg(p.own_len + req), 0), p.cache);
-    if (p.q_len) qlen = min(max(__ldg(p.q_len + req), 0), p.queries);
-  }
+  const int len = OWN ? own_length(p, req) : p.prefix;
+  const int qlen = OWN ? query_count(p, req) : p.queries;
   const int k0 = slot * p.chunk, k1 = min(len, k0 + p.chunk);
   const int64_t base = (int64_t)(OWN ? p.s1 + slot : slot) * p.rows;
-  auto row_at = [&](const Row& w) { return base + ((int64_t)w.r * p.queries + w.m) * p.heads + w.h; };
+  auto row_at = [&](const Row& w) { return base + row_index(p, w); };
   if (k0 >= k1) {   // nothing here: no output, a sum of zero
     if (threadIdx.x < 16 * WM) {
       const Row w = row_of<OWN>(p, tile * (16 * WM) + threadIdx.x, req, kh);
@@ -434,31 +405,74 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 
 // How a call is cut into items.
 struct Plan {
+  bool rows_run, tc_run;
   int wm1, rt1, s1, wm2, rt2, s2, chunk;
   int64_t items, rows;
+  TcPlan tc;
+  int64_t slots() const { return s1 + s2; }
+  bool joins() const { return !(tc_run && !rows_run && s1 == 1); }   // else outputs are written at once
+  int64_t bytes(int head_dim) const { return joins() ? slots() * rows * (head_dim + 2) * 4 : 0; }
 };
 
 static int warps_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
-static Plan make_plan(int requests, int queries, int heads, int kv_heads, int head_dim, int prefix, int cache) {
-  Plan p;
+// Chunks of key tiles per item of the tensor-core kernel: whole waves of 148
+// CTAs, each chunk with a few tiles' worth of start-up and end, against the
+// partial outputs that every chunk writes and the join reads.
+static int tc_splits(int64_t items, int64_t tiles, int64_t rows, int head_dim) {
+  const double tile_us = head_dim == 64 ? 1.5 : 2.2;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const double waves = (double)((items * s + 147) / 148);
+    double us = waves * ((double)((tiles + s - 1) / s) + 3) * tile_us;
+    if (s > 1) us += 4 + (double)s * rows * head_dim * 8 / 4e6;
+    if (s == 1 || us < least) {
+      least = us;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// joint, fold: whether the tensor-core kernel can take the call in that form.
+static Plan make_plan(int requests, int queries, int heads, int kv_heads, int head_dim, int prefix, int cache,
+                      bool joint, bool fold) {
+  Plan p{};
   const int group = heads / kv_heads;
   const int64_t r1 = (int64_t)requests * queries * group, r2 = (int64_t)queries * group;
   p.rows = r1 * kv_heads;
-  p.wm1 = warps_for(r1);
-  p.wm2 = warps_for(r2);
-  p.rt1 = (int)((r1 + p.wm1 * 16 - 1) / (p.wm1 * 16));
-  p.rt2 = (int)((r2 + p.wm2 * 16 - 1) / (p.wm2 * 16));
-  const int64_t t1 = (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
-  const int64_t units = kv_heads * (p.rt1 * t1 + (int64_t)requests * p.rt2 * t2);
-  // two items per resident CTA: short enough to even out requests of unequal
-  // lengths, long enough that the partial outputs are a small share
-  const int64_t want = 148ll * (head_dim == 64 ? 3 : 2) * 2;
-  const int64_t per = std::max<int64_t>((units + want - 1) / want, kSlotTiles);
-  p.chunk = (int)std::min<int64_t>(per, 1 << 24) * BN;
-  p.s1 = (int)((t1 + per - 1) / per);
-  p.s2 = (int)((t2 + per - 1) / per);
-  p.items = kv_heads * ((int64_t)p.rt1 * p.s1 + (int64_t)requests * p.rt2 * p.s2);
+  joint = joint && r2 > 64 && prefix + (int64_t)cache > 0;
+  fold = fold && !joint && r1 > 128 && prefix > 0;
+  p.tc_run = joint || fold;
+  p.rows_run = !joint && !(fold && cache == 0);
+  if (p.tc_run) {
+    p.tc.fold = fold;
+    p.tc.tokens = fold ? requests * queries : queries;
+    p.tc.per_tile = 128 / group;
+    p.tc.pairs = (p.tc.tokens + 2 * p.tc.per_tile - 1) / (2 * p.tc.per_tile);
+    const int64_t tiles = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
+    const int64_t items = (int64_t)p.tc.pairs * kv_heads * (fold ? 1 : requests);
+    const int s = tc_splits(items, tiles, p.rows, head_dim);
+    p.tc.per = (int)((tiles + s - 1) / s);
+    p.s1 = p.tc.splits = (int)((tiles + p.tc.per - 1) / p.tc.per);
+  }
+  if (p.rows_run) {
+    const int64_t t1 = p.tc_run ? 0 : (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
+    p.wm1 = p.tc_run ? 4 : warps_for(r1);
+    p.wm2 = warps_for(r2);
+    p.rt1 = p.tc_run ? 0 : (int)((r1 + p.wm1 * 16 - 1) / (p.wm1 * 16));
+    p.rt2 = (int)((r2 + p.wm2 * 16 - 1) / (p.wm2 * 16));
+    const int64_t units = kv_heads * (p.rt1 * t1 + (int64_t)requests * p.rt2 * t2);
+    // two items per resident CTA: short enough to even out requests of unequal
+    // lengths, long enough that the partial outputs are a small share
+    const int64_t want = 148ll * (head_dim == 64 ? 3 : 2) * 2;
+    const int64_t per = std::max<int64_t>((units + want - 1) / want, kSlotTiles);
+    p.chunk = (int)std::min<int64_t>(per, 1 << 24) * BN;
+    if (!p.tc_run) p.s1 = (int)((t1 + per - 1) / per);
+    p.s2 = (int)((t2 + per - 1) / per);
+    p.items = kv_heads * ((int64_t)p.rt1 * p.s1 + (int64_t)requests * p.rt2 * p.s2);
+  }
   return p;
 }
 
@@ -473,7 +487,8 @@ static int launch_rows(const Params& p, int64_t items, cudaStream_t st) {
 template <int D>
 static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
   int rc = GPA_OK;
-  if (plan.items > 0) {
+  if (plan.tc_run) rc = launch_tc(p, D, plan.tc, st);
+  if (!rc && plan.rows_run && plan.items > 0) {
     switch (plan.wm1 * 8 + plan.wm2) {   // wm2 <= wm1: own rows are part of the prefix's
       case 1 * 8 + 1: rc = launch_rows<D, 1, 1>(p, plan.items, st); break;
       case 2 * 8 + 1: rc = launch_rows<D, 2, 1>(p, plan.items, st); break;
@@ -483,7 +498,7 @@ static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
       default: rc = launch_rows<D, 4, 4>(p, plan.items, st); break;
     }
   }
-  if (rc) return rc;
+  if (rc || !plan.joins()) return rc;
   join_kernel<D><<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>(p);
   return check_launch("gpa_attention_shared_prefix");
 }
@@ -510,8 +525,12 @@ extern "C" int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int
                           prefix, cache))
     return -1;
   if (requests == 0 || queries == 0) return 0;
-  const prefix::Plan p = prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache);
-  return (int64_t)(p.s1 + p.s2) * p.rows * (head_dim + 2) * 4;
+  // strides decide which kernels can run: room for each way
+  int64_t bytes = 0;
+  for (int way = 0; way < 3; ++way)
+    bytes = std::max(bytes, prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache, way == 1,
+                                              way == 2).bytes(head_dim));
+  return bytes;
 }
 
 extern "C" int gpa_attention_shared_prefix(
@@ -534,11 +553,6 @@ extern "C" int gpa_attention_shared_prefix(
        o_sh | o_sm) & 7)
     return fail(GPA_ERR_INVALID, "%s: strides must be multiples of 8", what);
   if (!prefix_len) bias = nullptr;
-  const prefix::Plan plan = prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len);
-  if (plan.items >= (1ll << 31)) return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
-  const int64_t slots = plan.s1 + plan.s2;
-  if (slots && (!workspace || !aligned16(workspace) || workspace_bytes < slots * plan.rows * (head_dim + 2) * 4))
-    return fail(GPA_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
   prefix::Params p;
   p.q = (const __nv_bfloat16*)q;
   p.kp = (const __nv_bfloat16*)k_prefix;
@@ -560,16 +574,26 @@ extern "C" int gpa_attention_shared_prefix(
   p.ko_sr = ko_sr; p.ko_sh = ko_sh; p.ko_sn = ko_sn;
   p.vo_sr = vo_sr; p.vo_sh = vo_sh; p.vo_sn = vo_sn;
   p.bias_sh = bias_sh;
+  p.scale = sm_scale;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.causal = causal;
   p.o = (__nv_bfloat16*)o;
   p.o_sr = o_sr; p.o_sh = o_sh; p.o_sm = o_sm;
   p.lse = lse;
   p.lse_sr = lse_sr; p.lse_sh = lse_sh;
+  const prefix::Plan plan =
+      prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len,
+                        prefix::tc_takes(p, head_dim, false), prefix::tc_takes(p, head_dim, true));
+  if (plan.items >= (1ll << 31) || (int64_t)plan.tc.pairs * plan.tc.splits * kv_heads * requests >= (1ll << 31))
+    return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
+  const int64_t bytes = plan.bytes(head_dim);
+  if (bytes && (!workspace || !aligned16(workspace) || workspace_bytes < bytes))
+    return fail(GPA_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
+  p.status = status;
   p.rt1 = plan.rt1; p.s1 = plan.s1; p.rt2 = plan.rt2; p.s2 = plan.s2; p.chunk = plan.chunk;
   p.rows = plan.rows;
   p.ws_o = (float*)workspace;
-  p.ws_ml = reinterpret_cast<float2*>(p.ws_o + slots * plan.rows * head_dim);
+  p.ws_ml = reinterpret_cast<float2*>(p.ws_o + plan.slots() * plan.rows * head_dim);
   cudaStream_t st = (cudaStream_t)stream;
   return head_dim == 64 ? prefix::launch<64>(p, plan, st) : prefix::launch<128>(p, plan, st);
 }

@@ -1,0 +1,63 @@
+// What the kernels of the attention over a shared prefix have in common: the
+// call's parameters, the rows of a tile and the partial outputs of key chunks.
+#pragma once
+
+#include "common.cuh"
+#include "capi_util.h"
+
+namespace gpa {
+namespace prefix {
+
+struct Params {
+  const __nv_bfloat16 *q, *kp, *vp, *ko, *vo;
+  const float* bias;
+  const int32_t *own_len, *q_len;
+  int requests, queries, heads, kv_heads, group, prefix, cache;
+  int64_t q_sr, q_sh, q_sm, kp_sh, kp_sn, vp_sh, vp_sn, ko_sr, ko_sh, ko_sn, vo_sr, vo_sh, vo_sn, bias_sh;
+  float scale, scale_log2;
+  int causal;
+  __nv_bfloat16* o;
+  int64_t o_sr, o_sh, o_sm;
+  float* lse;
+  int64_t lse_sr, lse_sh;
+  // rows_kernel's items: row tiles x chunks of the prefix per key head, then of each request's cache
+  int rt1, s1, rt2, s2, chunk;   // chunk in keys; s1 + s2 partial outputs per row
+  int64_t rows;                  // requests * queries * heads
+  float* ws_o;                   // [s1 + s2][rows][D]
+  float2* ws_ml;                 // [s1 + s2][rows]: maximum (log2 units) and sum
+  int* status;
+};
+
+// One query row: request, token and query head.  Row i of a tile is query head
+// kh * group + i % group of token i / group.
+struct Row {
+  int r, m, h;
+  bool live;
+};
+
+__device__ __forceinline__ int64_t row_index(const Params& p, const Row& w) {
+  return ((int64_t)w.r * p.queries + w.m) * p.heads + w.h;
+}
+__device__ __forceinline__ int own_length(const Params& p, int r) {
+  return p.own_len ? min(max(__ldg(p.own_len + r), 0), p.cache) : p.cache;
+}
+__device__ __forceinline__ int query_count(const Params& p, int r) {
+  return p.q_len ? min(max(__ldg(p.q_len + r), 0), p.queries) : p.queries;
+}
+
+// The tensor-core kernel's share of a call: 2 x 128-row tiles over the prefix
+// and, unless `fold`, each request's own keys.
+struct TcPlan {
+  int fold;      // rows run through all requests (prefix only), else within one request
+  int tokens;    // tokens a tile's rows may come from: requests * queries (fold) or queries
+  int per_tile;  // tokens of a 128-row tile
+  int pairs;     // tile pairs over the tokens
+  int splits;    // chunks over the key tiles
+  int per;       // key tiles per chunk
+};
+// Whether the kernel can take the call's strides and scale.
+bool tc_takes(const Params& p, int head_dim, bool fold);
+int launch_tc(const Params& p, int head_dim, const TcPlan& t, cudaStream_t st);
+
+}  // namespace prefix
+}  // namespace gpa

@@ -127,6 +127,10 @@ SIZES = [
     (1, 600, 2, 2, 64, 1100, 700),
     (4, 129, 8, 2, 128, 0, 260),
     (2, 257, 3, 3, 64, 1025, 0),
+    (40, 9, 2, 2, 64, 700, 50),             # few rows each, many together
+    (150, 1, 3, 3, 128, 260, 5),
+    (33, 2, 8, 2, 64, 129, 0),
+    (20, 7, 6, 2, 128, 1500, 200),
 ]
 
 
@@ -136,7 +140,8 @@ def test_sizes(size, bias, causal):
     check(make(*size, bias=bias, causal=causal, seed=sum(size)))
 
 
-@pytest.mark.parametrize("size", [(6, 1, 4, 2, 64, 70, 300), (6, 5, 4, 4, 128, 70, 130), (6, 40, 2, 1, 64, 33, 200),
+@pytest.mark.parametrize("size", [(6, 1, 4, 2, 64, 70, 300), (6, 60, 3, 3, 64, 500, 90), (6, 50, 2, 2, 128, 0, 90),
+                                  (6, 5, 4, 4, 128, 70, 130), (6, 40, 2, 1, 64, 33, 200),
                                   (6, 140, 2, 1, 64, 300, 200), (6, 129, 2, 2, 128, 0, 140)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_lengths(size, causal):
@@ -234,6 +239,61 @@ def test_strided_views_and_in_place_buffers():
         a["k_own"] = a["k_own"][:1].expand(R, H, N, D)
         a["v_prefix"] = a["v_prefix"][:1].expand(H, P, D)
         check(a)
+
+
+@pytest.mark.parametrize("size", [(3, 1, 2, 2, 64, 200, 50), (3, 30, 2, 2, 128, 200, 50), (3, 150, 2, 2, 64, 200, 50),
+                                  (3, 150, 2, 2, 128, 200, 50), (30, 6, 2, 2, 64, 200, 50)])
+def test_nan_and_infinity_of_keys_that_count(size):
+    """A NaN or infinite score, in any key, makes its rows NaN and no others."""
+    R = size[0]
+    for key, value in [(0, float("nan")), (6, float("nan")), (7, INF), (13, -INF), (198, float("nan"))]:
+        a = make(*size, seed=8)
+        clean = run(a)
+        a["k_own"][1, 1, key % 50, 3] = value
+        a["k_prefix"][0, key, 5] = value
+        out, lse = run(a)
+        o, mag, ref, _ = reference(a)
+        ok = torch.ones(R, 2, dtype=torch.bool, device="cuda")
+        ok[:, 0] = False
+        ok[1, 1] = False
+        assert torch.equal(out[ok], clean[0][ok]) and torch.equal(lse[ok], clean[1][ok])
+        bad = torch.isnan(ref)           # an infinite key gives -inf to half of the queries: they stay finite
+        assert torch.equal(torch.isnan(lse), bad) and torch.equal(torch.isnan(out).any(-1), bad)
+        assert bool(torch.isnan(out)[bad].all())
+
+
+def test_values_that_are_not_finite():
+    """A NaN in V reaches its feature of every row that sees the key."""
+    for size in [(2, 1, 2, 2, 64, 200, 50), (2, 150, 2, 2, 128, 200, 50)]:
+        a = make(*size, seed=8)
+        clean, _ = run(a)
+        a["v_prefix"][1, 77, 9] = float("nan")
+        out, _ = run(a)
+        assert bool(torch.isnan(out[:, 1, :, 9]).all())
+        out[:, 1, :, 9] = clean[:, 1, :, 9]
+        assert torch.equal(out, clean)
+
+
+def test_queries_whose_requests_do_not_follow_on():
+    """Requests further apart than their tokens, or queries shared by all."""
+    for size in [(40, 4, 2, 2, 64, 300, 40), (3, 140, 2, 2, 128, 300, 40), (30, 1, 8, 1, 64, 300, 40)]:
+        R, M, H, Hk, D = size[:5]
+        a = make(*size, bias="key")
+        wide = torch.zeros(R, M + 1, H, D, device="cuda", dtype=BF16)
+        wide[:, :M] = a["q"].transpose(1, 2)
+        a["q"] = wide[:, :M].transpose(1, 2)
+        check(a)
+        a["q"] = a["q"][:1].expand(R, H, M, D)
+        check(a)
+
+
+def test_scales():
+    """Scales that are zero, negative or out of the ordinary."""
+    for M in (1, 200):
+        for scale in (0.0, -0.125, 1e-9, 1e-5):
+            a = make(2, M, 2, 2, 64, 300, 100, bias="key", causal=True)
+            a["sm_scale"] = scale
+            check(a)
 
 
 @pytest.mark.parametrize("M", [1, 40, 260])

@@ -76,10 +76,10 @@ def reference(a):
             if s.shape[1] == 0 or m == 0:
                 continue
             mx = s.amax(-1, keepdim=True)
-            mx = torch.where(mx > -INF, mx, torch.zeros_like(mx))
+            mx = torch.where(mx == -INF, torch.zeros_like(mx), mx)      # NaN stays
             e = torch.exp(s - mx)
             l = e.sum(-1, keepdim=True)
-            some = l > 0
+            some = l != 0
             p = torch.where(some, e / l, torch.zeros_like(e))
             o[r, h, :m], mag[r, h, :m] = p @ v, p @ v.abs()
             lse[r, h, :m] = torch.where(some, mx * math.log2(math.e) + torch.log2(l), torch.full_like(l, -INF))[:, 0]

@@ -134,6 +134,12 @@ def stream_of(t: torch.Tensor) -> _vp:
     return _vp(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device `index` as a cudaStream_t (the address
+    that current_stream wraps in an object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_cuda(*tensors, what: str) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -338,6 +338,7 @@ __device__ __forceinline__ void run_item(const Params& p, uint8_t* smem, int kh,
 template <int D, int WM1, int WM2>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
   // items of the prefix: row tile fastest (its CTAs share the keys in L2)
   int64_t it = blockIdx.x;
   const int64_t n1 = (int64_t)p.kv_heads * p.s1 * p.rt1;
@@ -355,52 +356,104 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   run_item<D, WM2, true>(p, smem, (int)(it % p.kv_heads), (int)(it / p.kv_heads), t, s);
 }
 
-// Joins a row's chunks: one warp per row.
-template <int D>
+// Joins a row's chunks.  W warps per row: one for a few chunks, eight (a block)
+// for many, each taking every eighth chunk.  The launch overlaps the end of the
+// kernel before it (a programmatic dependency), which the first line waits for.
+template <int D, int W>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  constexpr int F = D / 32;   // features per lane
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
   if (row >= p.rows) return;
-  const int h = (int)(row % p.heads);
-  const int64_t tok = row / p.heads;
-  const int m = (int)(tok % p.queries), r = (int)(tok / p.queries);
+  const int h = (int)((uint32_t)row % (uint32_t)p.heads), tok = (int)((uint32_t)row / (uint32_t)p.heads);
+  const int m = (int)((uint32_t)tok % (uint32_t)p.queries), r = (int)((uint32_t)tok / (uint32_t)p.queries);
   if (p.q_len && m >= __ldg(p.q_len + r)) return;
   const int slots = p.s1 + p.s2;
-  float mx = -INFINITY;
-  for (int s = lane; s < slots; s += 32) mx = fmaxf(mx, p.ws_ml[(int64_t)s * p.rows + row].x);
+  const float2* mlr = p.ws_ml + row;
+  const float2 first = lane < slots ? mlr[lane * p.rows] : make_float2(-INFINITY, 0.f);
+  float mx = first.x;
+  for (int s = lane + 32; s < slots; s += 32) mx = fmaxf(mx, mlr[s * p.rows].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float l = 0.f, v[D / 32];
+  float l = 0.f, v[F];
 #pragma unroll
-  for (int u = 0; u < D / 32; ++u) v[u] = 0.f;
+  for (int u = 0; u < F; ++u) v[u] = 0.f;
+  const float* orow = p.ws_o + row * D + lane * F;
   for (int s0 = 0; s0 < slots; s0 += 32) {
-    float f = 0.f;
-    if (s0 + lane < slots) {
-      const float2 ml = p.ws_ml[(int64_t)(s0 + lane) * p.rows + row];
-      f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
-      l = fmaf(ml.y, f, l);
-    }
+    const float2 ml = s0 == 0 ? first : (s0 + lane < slots ? mlr[(s0 + lane) * p.rows] : make_float2(-INFINITY, 0.f));
+    const float f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
+    l = fmaf(ml.y, f, l);
     const int n = min(32, slots - s0);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, i);
-      if (w > 0.f) {   // an empty chunk wrote no output
-        const float* o = p.ws_o + ((int64_t)(s0 + i) * p.rows + row) * D + lane * (D / 32);
+    constexpr int U = 8;   // loads in flight
+    for (int i0 = W == 1 ? 0 : warp; i0 < n; i0 += U * W) {
+      float x[U][F], w[U];
 #pragma unroll
-        for (int u = 0; u < D / 32; ++u) v[u] = fmaf(w, o[u], v[u]);
+      for (int i = 0; i < U; ++i) {
+        const int s = i0 + i * W;
+        w[i] = __shfl_sync(0xffffffffu, f, s & 31);
+        if (s >= n) w[i] = 0.f;
+        const float* src = orow + (int64_t)(s0 + s) * p.rows * D;
+        if (w[i] > 0.f) {   // an empty chunk wrote no output
+          if constexpr (F == 2) {
+            const float2 t = *reinterpret_cast<const float2*>(src);
+            x[i][0] = t.x; x[i][1] = t.y;
+          } else {
+            const float4 t = *reinterpret_cast<const float4*>(src);
+            x[i][0] = t.x; x[i][1] = t.y; x[i][2] = t.z; x[i][3] = t.w;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < F; ++u) x[i][u] = 0.f;
+        }
       }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int u = 0; u < F; ++u) v[u] = fmaf(w[i], x[i][u], v[u]);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if constexpr (W > 1) {
+    __shared__ float part[W][D];
+#pragma unroll
+    for (int u = 0; u < F; ++u) part[warp][lane * F + u] = v[u];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int u = 0; u < F; ++u) {
+      v[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[u] += part[i][lane * F + u];
+    }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
-  __nv_bfloat16* orow = p.o + r * p.o_sr + h * p.o_sh + m * p.o_sm + lane * (D / 32);
-  if constexpr (D == 64) {
-    *reinterpret_cast<uint32_t*>(orow) = pack_bf16x2(v[0] * inv, v[1] * inv);
+  __nv_bfloat16* dst = p.o + r * p.o_sr + h * p.o_sh + m * p.o_sm + lane * F;
+  if constexpr (F == 2) {
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(v[0] * inv, v[1] * inv);
   } else {
-    *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
   }
   if (p.lse && lane == 0) p.lse[r * p.lse_sr + h * p.lse_sh + m] = l == 0.f ? -INFINITY : mx + log2f(l);
+}
+
+template <int D>
+static int launch_join(const Params& p, cudaStream_t st) {
+  // eight warps per row from where one would go twice through its eight loads
+  const bool wide = p.s1 + p.s2 > 16;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(wide ? p.rows : (p.rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, join_kernel<D, 8>, p) : cudaLaunchKernelEx(&cfg, join_kernel<D, 1>, p);
+  if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
+  return check_launch("gpa_attention_shared_prefix");
 }
 
 // How a call is cut into items.
@@ -499,8 +552,7 @@ static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
     }
   }
   if (rc || !plan.joins()) return rc;
-  join_kernel<D><<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>(p);
-  return check_launch("gpa_attention_shared_prefix");
+  return launch_join<D>(p, st);
 }
 
 static int check_sizes(const char* what, int requests, int queries, int heads, int kv_heads, int head_dim, int prefix,

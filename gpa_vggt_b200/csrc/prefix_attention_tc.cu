@@ -66,6 +66,9 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
+// The two softmax warpgroups.
+__device__ __forceinline__ void named_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
 // 2 of 8 exponentials on the FMA pipe, the rest on MUFU
 __device__ __forceinline__ void exp8(const float* x, float* e) {
 #pragma unroll
@@ -81,6 +84,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   using SM = TcSmem<D>;
   constexpr int ST = SM::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
 
   // the item: row tiles fastest, then requests, so that CTAs running together
   // read the same keys of the prefix
@@ -103,6 +107,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   const int tp = (p.prefix + TM - 1) / TM;
   const int j0 = split * tc.per;
   const int nk = max(0, min(tp + (own_end + TM - 1) / TM, j0 + tc.per) - j0);
+  // Two streams of work for the issuers and softmax warpgroups: the two row
+  // tiles over the same key tiles, or, where only one has rows, that one over the
+  // even and the odd key tiles (joined at the end).
+  const bool halves = active == 1 && nk > 1;
+  const int streams = nk > 1 ? 2 : active;
   const bool partial = p.s1 + p.s2 > 1;
   auto row_of = [&](int t, int i) {
     Row w;
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       bar_init(&v_full[s], 1);
       bar_init(&k_ok[s], 1);
       bar_init(&v_ok[s], 1);
-      bar_init(&k_empty[s], active);   // one arrival per row tile's issuer
+      bar_init(&k_empty[s], active);   // one arrival per stream that reads the tile
       bar_init(&v_empty[s], active);
     }
     for (int t = 0; t < 2; ++t) {
@@ -308,21 +317,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (any) zero_rows(smem + SM::V + s * SM::TILE);
         if (lane == 0) bar_arrive(&v_ok[s]);
       }
-    } else if (warp - 1 < active) {
+    } else if (warp - 1 < streams) {
       // ------------------------------ MMA issuers ------------------------------
+      // j counts this stream's key tiles, key_tile(j) the chunk's
       const int t = warp - 1;
+      const int n = halves ? (nk - t + 1) >> 1 : nk;
+      auto key_tile = [&](int j) { return halves ? 2 * j + t : j; };
       const bool leader = elect_one();
       constexpr uint32_t idesc_s = idesc_bf16(TM, TM, false, false);
       constexpr uint32_t idesc_o = idesc_bf16(TM, D, false, true);
-      const uint64_t dQ = sdesc_sw128(smem_u32(smem + SM::Q + t * SM::TILE), 16, 1024);
+      const uint64_t dQ = sdesc_sw128(smem_u32(smem + SM::Q + (halves ? 0 : t) * SM::TILE), 16, 1024);
       const uint64_t dK = sdesc_sw128(smem_u32(smem + SM::K), 16, 1024);
       const uint64_t dV = sdesc_sw128(smem_u32(smem + SM::V), SM::HALF, 1024);
       const uint64_t dOnes = sdesc_plain(smem_u32(smem + SM::ONES));
       const uint64_t dBeta = sdesc_plain(smem_u32(smem + SM::BETA));
       const uint32_t dS = tbase + col_s(t), dO = tbase + col_o(t), dP = tbase + col_p(t);
       auto issue_s = [&](int j) {
-        const int st = j % ST;
-        const bool beta = has_beta(tile_of(j));
+        const int jt = key_tile(j), st = jt % ST;
+        const bool beta = has_beta(tile_of(jt));
         if (leader) {
           const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
@@ -337,7 +349,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
       };
       auto issue_o = [&](int j) {
-        const int st = j % ST;
+        const int st = key_tile(j) % ST;
         if (leader) {
           const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
@@ -348,25 +360,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         __syncwarp();
       };
-      bool okw = wait(q_full, 0) && wait(&k_ok[0], 0);
+      auto wait_tile = [&](uint64_t* bar, int j) { return wait(&bar[key_tile(j) % ST], key_tile(j) / ST); };
+      bool okw = wait(q_full, 0) && wait_tile(k_ok, 0);
       if (okw) {
         tc_fence_after();
         issue_s(0);
       }
-      for (int j = 0; okw && j < nk; ++j) {
-        if (D == 64 && j + 1 < nk) {
-          okw = wait(&s_empty[t], j) && wait(&k_ok[(j + 1) % ST], (j + 1) / ST);
+      for (int j = 0; okw && j < n; ++j) {
+        if (D == 64 && j + 1 < n) {
+          okw = wait(&s_empty[t], j) && wait_tile(k_ok, j + 1);
           if (!okw) break;
           tc_fence_after();
           issue_s(j + 1);
         }
-        okw = wait(&p_full[t], j) && wait(&v_ok[j % ST], j / ST);
+        okw = wait(&p_full[t], j) && wait_tile(v_ok, j);
         if (!okw) break;
         tc_fence_after();
         issue_o(j);
-        if (D == 128 && j + 1 < nk) {
+        if (D == 128 && j + 1 < n) {
           // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
-          okw = wait(&k_ok[(j + 1) % ST], (j + 1) / ST) && wait(&o_done[t], j);
+          okw = wait_tile(k_ok, j + 1) && wait(&o_done[t], j);
           if (!okw) break;
           tc_fence_after();
           issue_s(j + 1);
@@ -377,11 +390,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     regs_inc<TC_HIGH>();
     // ------------------------------ softmax ------------------------------
     const int t = (warp - 4) >> 2;
-    if (t < active) {
+    if (t < streams) {
+      const int n = halves ? (nk - t + 1) >> 1 : nk;
       const int quad = warp & 3;
       const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
       const uint32_t tS = tbase + lane_off + col_s(t), tO = tbase + lane_off + col_o(t), tP = tbase + lane_off + col_p(t);
-      const Row row = row_of(t, quad * 32 + lane);
+      const Row row = row_of(halves ? 0 : t, quad * 32 + lane);
+      const bool idle = !__any_sync(0xffffffffu, row.live);   // a warp without rows only keeps the barriers going
       // own keys that this row sees end here
       const int limit = p.causal && !tc.fold ? len - qlen + row.m + 1 : 0x7fffffff;
       float m_raw = -INFINITY, l = 0.f;   // running maximum (score units), row sum
@@ -401,9 +416,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           for (int i = 0; i < 4; ++i) pk[g * 4 + i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
         }
       };
-      for (int j = 0; j < nk; ++j) {
+      for (int j = 0; j < n; ++j) {
         if (!wait(&s_full[t], j)) { okw = false; break; }
         tc_fence_after();
+        if (idle) {
+          // S(j+1) may be there before the other warps' P(j): no second arrival in one phase
+          if (j > 0 && !wait(&p_full[t], j - 1)) { okw = false; break; }
+          if (lane == 0) {
+            if (D == 64) bar_arrive(&s_empty[t]);
+            bar_arrive(&p_full[t]);
+          }
+          continue;
+        }
         float x[TM];
 #pragma unroll
         for (int c = 0; c < TM / 32; ++c) tmem_ld32f(tS + c * 32, x + c * 32);
@@ -411,7 +435,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
-        const Tile kt = tile_of(j);
+        const Tile kt = tile_of(halves ? 2 * j + t : j);
         if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {   // keys ahead of this row
           const int end = limit - kt.key0;
 #pragma unroll
@@ -478,10 +502,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(&p_full[t]);
       }
-      if (okw) okw = wait(&o_done[t], nk - 1);
-      if (okw && !*abort_flag) {
-        tc_fence_after();
-        const bool some = m_raw > -INFINITY || l != l;   // else the sum holds the polynomial's 2^-126
+      if (okw) okw = wait(&o_done[t], n - 1);
+      tc_fence_after();
+      // The second half's output goes through the rings' memory (all of it has
+      // been read once both halves are done), feature-major: a thread per row.
+      float* xo = reinterpret_cast<float*>(smem + SM::K) + quad * 32 + lane;
+      float* xml = reinterpret_cast<float*>(smem + SM::Q) + (quad * 32 + lane) * 2;
+      float f1 = 0.f;
+      if (halves) {
+        named_sync();
+        if (t == 1 && okw) {
+          xml[0] = m_raw;
+          xml[1] = l;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t ov[32];
+            tmem_ld32(tO + c * 32, ov);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) xo[(c * 32 + i) * TM] = __uint_as_float(ov[i]);
+          }
+        }
+        named_sync();
+      }
+      if (okw && !*abort_flag && !(halves && t == 1)) {
+        float f0 = 1.f;
+        if (halves) {
+          const float m1 = xml[0], m = fmaxf(m_raw, m1);
+          const bool any = m > -INFINITY;   // else the sums hold the polynomial's 2^-126, or a NaN
+          f0 = any ? fast_exp2((m_raw - m) * c2) : 1.f;
+          f1 = any ? fast_exp2((m1 - m) * c2) : 1.f;
+          l = l * f0 + xml[1] * f1;
+          m_raw = m;
+        }
+        const bool some = m_raw > -INFINITY || l != l;
         const float inv = some ? 1.0f / l : 0.f;
         const int64_t at = split * p.rows + row_index(p, row);
         __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
@@ -491,17 +545,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           tmem_ld32(tO + c * 32, ov);
           tmem_wait_ld();
           if (!row.live) continue;
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ov[i]);
+          if (halves) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], f0, xo[(c * 32 + i) * TM] * f1);
+          }
           if (partial) {
             float4* w = reinterpret_cast<float4*>(p.ws_o + at * D + c * 32);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              w[u] = make_float4(__uint_as_float(ov[4 * u]), __uint_as_float(ov[4 * u + 1]),
-                                 __uint_as_float(ov[4 * u + 2]), __uint_as_float(ov[4 * u + 3]));
+            for (int u = 0; u < 8; ++u) w[u] = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
           } else {
             uint32_t w[16];
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-              w[u] = some ? pack_bf16x2(__uint_as_float(ov[2 * u]) * inv, __uint_as_float(ov[2 * u + 1]) * inv) : 0u;
+            for (int u = 0; u < 16; ++u) w[u] = some ? pack_bf16x2(v[2 * u] * inv, v[2 * u + 1] * inv) : 0u;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
               reinterpret_cast<uint4*>(orow + c * 32)[u] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);

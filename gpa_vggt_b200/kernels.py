@@ -113,6 +113,61 @@ def _tma_ok(t: torch.Tensor) -> bool:
     return all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
 
 
+_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+_DTYPES = {F32: _lib.GPA_DTYPE_F32, BF16: _lib.GPA_DTYPE_BF16}
+
+
+def _one_device(first: torch.Tensor, *others, what: str) -> int:
+    """Index of the CUDA device that holds every given tensor."""
+    index = first.get_device()
+    if index < 0:
+        require_cuda(first, what=what)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            require_cuda(t, what=what)
+            raise ValueError(f"{what}: tensors are on different devices")
+    return index
+
+
+def _on(index: int):
+    """Make device `index` current for a launch on one of its streams."""
+    if index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _rows(t: torch.Tensor, cols: int):
+    """(t or a copy of it, row stride): [rows, cols] in memory, 16-byte aligned
+    rows of contiguous elements; a view wherever t allows it."""
+    if t.is_contiguous() and aligned(t):
+        return t, cols
+    t2 = t.reshape(t.numel() // cols, cols)
+    ld = t2.stride(0) if t2.shape[0] > 1 else cols      # a single row's stride says nothing
+    if t2.stride(1) != 1 or ld % 8 or not aligned(t2):
+        t2, ld = t2.clone(memory_format=torch.contiguous_format), cols
+    return t2, ld
+
+
+def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and 16-byte aligned."""
+    if t is None or (t.is_contiguous() and aligned(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _fresh_like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape and type (empty_like is the cheapest
+    allocation, but keeps the strides of a permuted tensor)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 def sim_argmax(a: torch.Tensor, b: torch.Tensor, status: Optional[torch.Tensor] = None):
     """node_max [B,M] fp32, node_idx [B,M] int32 of a [B,M,D] vs b [B,N,D] (bf16)."""
     require_cuda(a, b, what="sim_argmax")
@@ -402,9 +457,18 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
     return (out, lse) if return_lse else out
 
 
-def _kernel_strides(t: torch.Tensor):
-    """Strides of all dims but the last, 0 where a dim has at most one entry."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+def _vectors(t: torch.Tensor):
+    """(t or a copy of it, strides of all dims but the last, 0 where a dim has at
+    most one entry): innermost dim contiguous, 16-byte aligned vectors."""
+    if t.is_contiguous():
+        if aligned(t):
+            return t, t.stride()[:-1]
+    else:
+        strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+        if t.stride(-1) == 1 and aligned(t) and not any(s % 8 for s in strides[:-1]):
+            return t, strides[:-1]
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:-1]
 
 
 def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out):
@@ -413,35 +477,37 @@ def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bi
         raise ValueError(f"{what}: q [R,H,M,D], k_prefix [Hk,P,D] and k_own [R,Hk,N,D] required")
     R, H, M, D = q.shape
     Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]
-    if (tuple(v_prefix.shape) != (Hk, P, D) or tuple(k_prefix.shape) != (Hk, P, D)
-            or tuple(k_own.shape) != (R, Hk, N, D) or tuple(v_own.shape) != (R, Hk, N, D)):
+    if (k_prefix.shape != (Hk, P, D) or v_prefix.shape != (Hk, P, D) or k_own.shape != (R, Hk, N, D)
+            or v_own.shape != (R, Hk, N, D)):
         raise ValueError(f"{what}: keys and values do not fit q [R,H,M,D]: [Hk,P,D] and [R,Hk,N,D] required")
-    if any(t.dtype != BF16 for t in (q, k_prefix, v_prefix, k_own, v_own)):
-        raise TypeError(f"{what}: q, keys and values must be bf16")
-    if D not in (64, 128):
+    for t in (q, k_prefix, v_prefix, k_own, v_own):
+        if t.dtype != BF16:
+            raise TypeError(f"{what}: q, keys and values must be bf16")
+    if D != 64 and D != 128:
         raise ValueError(f"{what}: head dim 64 or 128 required")
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{what}: the query heads must be a multiple of the key heads")
     for t in (own_len, q_len):
-        if t is not None and t.dtype != torch.int32:
-            raise TypeError(f"{what}: own_len and q_len must be int32")
-        if t is not None and tuple(t.shape) != (R,):
-            raise ValueError(f"{what}: own_len and q_len must be [R]")
+        if t is not None:
+            if t.dtype != torch.int32:
+                raise TypeError(f"{what}: own_len and q_len must be int32")
+            if t.shape != (R,):
+                raise ValueError(f"{what}: own_len and q_len must be [R]")
     if bias is not None:
         if not bias.is_floating_point():
             raise TypeError(f"{what}: bias must be a floating type")
-        if bias.dim() not in (1, 2) or bias.shape[-1] != P or (bias.dim() == 2 and bias.shape[0] not in (1, Hk)):
+        if bias.shape != (P,) and bias.shape != (1, P) and bias.shape != (Hk, P):
             raise ValueError(f"{what}: bias must be [P], [1,P] or [Hk,P]")
-    if out is not None and (out.dtype != BF16 or tuple(out.shape) != (R, H, M, D)
-                            or (out.numel() and not _tma_ok(out))):
+    if out is not None and (out.dtype != BF16 or out.shape != q.shape or (out.numel() and _vectors(out)[0] is not out)):
         raise ValueError(f"{what}: out must be a bf16 [R,H,M,D] view, innermost contiguous, 16-byte aligned rows")
-    if lse_out is not None and (lse_out.dtype != F32 or tuple(lse_out.shape) != (R, H, M)
+    if lse_out is not None and (lse_out.dtype != F32 or lse_out.shape != (R, H, M)
                                 or (M > 1 and lse_out.stride(-1) != 1)):
         raise ValueError(f"{what}: lse_out must be an fp32 [R,H,M] view with row stride 1")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k_prefix, v_prefix, k_own, v_own, bias)):
-        raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
-    return _device_of(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, what=what)
+    if torch.is_grad_enabled():
+        for t in (q, k_prefix, v_prefix, k_own, v_own, bias):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
+    return _one_device(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, what=what)
 
 
 def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
@@ -468,18 +534,23 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
     -inf.  Nothing is read back to the host, so calls can be captured; no
     gradients."""
-    device = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out)
+    index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out)
     R, H, M, D = q.shape
     Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]
+    device = q.device
     if out is None:
-        out = (torch.empty if q_len is None else torch.zeros)(R, H, M, D, device=device, dtype=BF16)
+        out = (torch.empty if q_len is None else torch.zeros)((R, H, M, D), device=device, dtype=BF16)
     if lse_out is None and return_lse:
-        lse_out = (torch.empty(R, H, M, device=device, dtype=F32) if q_len is None
+        lse_out = (torch.empty((R, H, M), device=device, dtype=F32) if q_len is None
                    else torch.full((R, H, M), -float("inf"), device=device, dtype=F32))
     if R * M == 0:
         return (out, lse_out) if lse_out is not None else out
-    q, k_prefix, v_prefix, k_own, v_own = (t if _tma_ok(t) else t.clone(memory_format=torch.contiguous_format)
-                                           for t in (q, k_prefix, v_prefix, k_own, v_own))
+    q, qs = _vectors(q)
+    k_prefix, kps = _vectors(k_prefix)
+    v_prefix, vps = _vectors(v_prefix)
+    k_own, kos = _vectors(k_own)
+    v_own, vos = _vectors(v_own)
+    os = _vectors(out)[1]
     bias_sh = 0
     if bias is not None:
         bias = bias.detach().to(F32)
@@ -489,15 +560,14 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
             bias_sh = bias.stride(0)
     own_len, q_len = (None if t is None else t.contiguous() for t in (own_len, q_len))
     size = _lib.load().gpa_attention_shared_prefix_workspace_bytes(R, M, H, Hk, D, P, N)
-    ws = torch.empty(max(size, 16), device=device, dtype=torch.uint8)
+    ws = torch.empty(size, device=device, dtype=torch.uint8) if size > 0 else None
     status, own = _status_word(status, device)
     ls = (0, 0) if lse_out is None else lse_out.stride()[:2]
-    with _on(device):
-        call("gpa_attention_shared_prefix", ptr(q), *_kernel_strides(q), ptr(k_prefix), *_kernel_strides(k_prefix),
-             ptr(v_prefix), *_kernel_strides(v_prefix), ptr(bias), bias_sh, ptr(k_own), *_kernel_strides(k_own),
-             ptr(v_own), *_kernel_strides(v_own), ptr(own_len), ptr(q_len), R, M, H, Hk, D, P, N, float(sm_scale),
-             int(bool(causal)), ptr(out), *_kernel_strides(out), ptr(lse_out), *ls, ptr(ws), size, ptr(status),
-             stream_of(q))
+    with _on(index):
+        call("gpa_attention_shared_prefix", q.data_ptr(), *qs, _address(k_prefix), *kps, _address(v_prefix), *vps,
+             _address(bias), bias_sh, _address(k_own), *kos, _address(v_own), *vos, _address(own_len),
+             _address(q_len), R, M, H, Hk, D, P, N, sm_scale, 1 if causal else 0, out.data_ptr(), *os,
+             _address(lse_out), *ls, _address(ws), size, status.data_ptr(), _lib.raw_stream(index))
     if own:
         _check_status(status, "gpa_attention_shared_prefix")
     return (out, lse_out) if lse_out is not None else out
@@ -629,67 +699,69 @@ def residual_scale(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     return out
 
 
-_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
-
-
-def _device_of(*tensors, what: str):
-    """The one CUDA device of the given tensors."""
-    require_cuda(*tensors, what=what)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"{what}: tensors are on different devices")
-    return devices.pop()
-
-
-def _on(device):
-    """Make `device` current for a launch on one of its streams."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """[rows, cols] with 16-byte aligned rows (a view where t allows it)."""
-    t2 = t.reshape(t.numel() // cols, cols)
-    if t2.stride(-1) != 1 or t2.stride(0) % 8 or not aligned(t2):
-        t2 = t2.contiguous()
-        if not aligned(t2):
-            t2 = t2.clone()
-    return t2
-
-
-def _ld(t2: torch.Tensor) -> int:
-    """Row stride of _rows' result (a single row's stride says nothing)."""
-    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
-
-
-def _param(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """Contiguous and 16-byte aligned."""
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t if aligned(t) else t.clone()
-
-
 def _residual_norm_launch(x, y, gate, weight, bias, post_weight, post_bias, eps, kind, post_kind, post_eps,
                           want_stats):
-    C = x.shape[-1]
+    shape, index, dtype = x.shape, x.get_device(), x.dtype
+    C = shape[-1]
     rows = x.numel() // C
-    z = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    h = None if kind is None else torch.empty(x.shape, device=x.device, dtype=y.dtype)
+    z = _fresh_like(x)
+    h = None if kind is None else _fresh_like(y)
     stats = torch.empty(rows, 4, device=x.device, dtype=F32) if want_stats else None
     if rows == 0:
         return z, h, stats
-    x2, y2, gate = _rows(x, C), _rows(y, C), _param(gate)
-    weight, bias, post_weight, post_bias = (_param(t) for t in (weight, bias, post_weight, post_bias))
-    first = next((t for t in (weight, bias, post_weight, post_bias) if t is not None), None)
-    with _on(x.device):
-        call("gpa_residual_norm", ptr(x2), _dt(x), _ld(x2), ptr(y2), _dt(y), _ld(y2), ptr(gate),
-             0 if gate is None else _dt(gate), 0 if gate is None else rows // (gate.numel() // C), rows, C,
-             _NORM_KINDS[post_kind], ptr(post_weight), ptr(post_bias), post_eps, _NORM_KINDS[kind],
-             ptr(weight), ptr(bias), 0 if first is None else _dt(first), eps, ptr(z), C, ptr(h), C, ptr(stats),
-             stream_of(x))
+    x, xs = _rows(x, C)
+    y, ys = _rows(y, C)
+    gate_dtype = gate_rows = param_dtype = 0
+    if gate is not None:
+        gate, gate_dtype, gate_rows = _param(gate), _DTYPES[gate.dtype], rows // (gate.numel() // C)
+    params = []
+    for t in (post_weight, post_bias, weight, bias):
+        if t is not None:
+            param_dtype = _DTYPES[t.dtype]
+        params.append(_param(t))
+    pw, pb, w, b = params
+    with _on(index):
+        call("gpa_residual_norm", x.data_ptr(), _DTYPES[dtype], xs, y.data_ptr(), _DTYPES[y.dtype], ys, _address(gate),
+             gate_dtype, gate_rows, rows, C, _NORM_KINDS[post_kind], _address(pw), _address(pb), post_eps,
+             _NORM_KINDS[kind], _address(w), _address(b), param_dtype, eps, z.data_ptr(), C, _address(h), C,
+             _address(stats), _lib.raw_stream(index))
     return z, h, stats
+
+
+def _residual_norm_gradients(ctx, dz, dh=None):
+    z, y, gate, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
+    kind, post_kind = ctx.kinds
+    C = z.shape[-1]
+    rows = z.numel() // C
+    params = (gate, weight, bias, post_weight, post_bias)
+    if (dz is None and dh is None) or rows == 0:
+        return (*(None if t is None else torch.zeros_like(t) for t in (z, y, *params)), None, None, None, None)
+    dx, dy = _fresh_like(z), _fresh_like(y)
+    grads = [_fresh_like(t) if t is not None and need else None
+             for t, need in zip(params, ctx.needs_input_grad[2:7])]
+    dzs = dhs = gate_dtype = param_dtype = 0
+    if dz is not None:
+        dz, dzs = _rows(dz, C)
+    if dh is not None:
+        dh, dhs = _rows(dh, C)
+    y, ys = _rows(y, C)
+    gate_rows = rows
+    if gate is not None:
+        gate, gate_dtype, gate_rows = _param(gate), _DTYPES[gate.dtype], rows // (gate.numel() // C)
+    for t in params[1:]:
+        if t is not None:
+            param_dtype = _DTYPES[t.dtype]
+    weight, post_weight, post_bias = _param(weight), _param(post_weight), _param(post_bias)
+    size = _lib.load().gpa_residual_norm_backward_workspace_bytes(rows, C, gate_rows)
+    ws = torch.empty(size, device=z.device, dtype=torch.uint8)
+    index = z.get_device()
+    with _on(index):
+        call("gpa_residual_norm_backward", _address(dz), dzs, _address(dh), dhs, z.data_ptr(), _DTYPES[z.dtype], C,
+             y.data_ptr(), _DTYPES[y.dtype], ys, stats.data_ptr(), _address(gate), gate_dtype, gate_rows, rows, C,
+             _NORM_KINDS[post_kind], _address(post_weight), _address(post_bias), _NORM_KINDS[kind], _address(weight),
+             param_dtype, dx.data_ptr(), C, dy.data_ptr(), C, *map(_address, grads), ws.data_ptr(), size,
+             _lib.raw_stream(index))
+    return (dx, dy, *grads, None, None, None, None)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -700,51 +772,27 @@ class _ResidualNorm(torch.autograd.Function):
         z, h, stats = _residual_norm_launch(x, y, gate, weight, bias, post_weight, post_bias, eps, kind,
                                             post_kind, post_eps, True)
         ctx.kinds = (kind, post_kind)
-        # the norms' own biases enter no gradient but their types do
         ctx.save_for_backward(z, y, gate, weight, bias, post_weight, post_bias, stats)
         ctx.set_materialize_grads(False)
         return z if h is None else (z, h)
 
+    # with create_graph, the gradients' own gradients are refused
+    _once = staticmethod(torch.autograd.function.once_differentiable(_residual_norm_gradients))
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dz, dh=None):
-        z, y, gate, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
-        kind, post_kind = ctx.kinds
-        C = z.shape[-1]
-        rows = z.numel() // C
-        params = (gate, weight, bias, post_weight, post_bias)
-        if (dz is None and dh is None) or rows == 0:
-            return (*(None if t is None else torch.zeros_like(t) for t in (z, y, *params)),
-                    None, None, None, None)
-        if dz is not None:
-            dz = _rows(dz, C)
-        if dh is not None:
-            dh = _rows(dh, C)
-        y2, gate_c = _rows(y, C), _param(gate)
-        dx, dy = torch.empty_like(z), torch.empty(y.shape, device=y.device, dtype=y.dtype)
-        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) if t is not None and need else None
-                 for t, need in zip(params, ctx.needs_input_grad[2:7])]
-        gate_rows = rows if gate is None else rows // (gate.numel() // C)
-        first = next((t for t in params[1:] if t is not None), None)
-        weight, post_weight, post_bias = _param(weight), _param(post_weight), _param(post_bias)
-        size = _lib.load().gpa_residual_norm_backward_workspace_bytes(rows, C, gate_rows)
-        ws = torch.empty(size, device=z.device, dtype=torch.uint8)
-        with _on(z.device):
-            call("gpa_residual_norm_backward", ptr(dz), 0 if dz is None else _ld(dz), ptr(dh),
-                 0 if dh is None else _ld(dh), ptr(z), _dt(z), C, ptr(y2), _dt(y), _ld(y2), ptr(stats),
-                 ptr(gate_c), 0 if gate is None else _dt(gate), gate_rows, rows, C, _NORM_KINDS[post_kind],
-                 ptr(post_weight), ptr(post_bias), _NORM_KINDS[kind], ptr(weight),
-                 0 if first is None else _dt(first), ptr(dx), C, ptr(dy), C, *(ptr(t) for t in grads), ptr(ws),
-                 size, stream_of(z))
-        return (dx, dy, *grads, None, None, None, None)
+    def backward(ctx, *grads):
+        if torch.is_grad_enabled():
+            return _ResidualNorm._once(ctx, *grads)
+        return _residual_norm_gradients(ctx, *grads)
 
 
 def _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind, post_kind):
-    if x.dim() < 1 or x.shape != y.shape:
+    shape = x.shape
+    if len(shape) < 1 or shape != y.shape:
         raise ValueError("residual_norm: x and y must have one shape [..., C]")
-    if (x.dtype, y.dtype) not in ((BF16, BF16), (F32, BF16), (F32, F32)):
+    dtype, y_dtype, C = x.dtype, y.dtype, shape[-1]
+    if dtype not in _DTYPES or not (y_dtype == dtype or y_dtype == BF16):
         raise TypeError("residual_norm: x and y must be bf16 or fp32, y no wider than x")
-    C = x.shape[-1]
     if C < 8 or C % 8 or C > 8192:
         raise ValueError("residual_norm: the last dim must be a multiple of 8, at most 8192")
     if x.numel() // C >= 2 ** 31:
@@ -754,23 +802,33 @@ def _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind,
     if (kind is None and (weight is not None or bias is not None)) or (
             post_kind is None and (post_weight is not None or post_bias is not None)):
         raise ValueError("residual_norm: parameters of a norm that is off")
-    params = [t for t in (weight, bias, post_weight, post_bias) if t is not None]
-    if any(tuple(t.shape) != (C,) for t in params):
-        raise ValueError("residual_norm: norm weights and biases must be [C]")
-    if any(t.dtype not in (F32, BF16) or t.dtype != params[0].dtype for t in params):
-        raise TypeError("residual_norm: norm weights and biases must all be bf16 or all fp32")
+    param_dtype = None
+    for t in (weight, bias, post_weight, post_bias):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != C:
+            raise ValueError("residual_norm: norm weights and biases must be [C]")
+        if t.dtype not in _DTYPES or (param_dtype is not None and t.dtype != param_dtype):
+            raise TypeError("residual_norm: norm weights and biases must all be bf16 or all fp32")
+        param_dtype = t.dtype
     if gate is not None:
-        if gate.dtype not in (F32, BF16):
+        if gate.dtype not in _DTYPES:
             raise TypeError("residual_norm: gate must be bf16 or fp32")
-        lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
-        n = len(lead)
-        while n and lead[n - 1] == 1:
-            n -= 1
-        if gate.dim() < 1 or gate.shape[-1] != C or (gate.dim() > 1 and (gate.dim() != x.dim()
-                                                                        or lead[:n] != full[:n])):
+        g = gate.shape
+        if len(g) < 1 or g[-1] != C or (len(g) > 1 and not _leads(g[:-1], shape[:-1])):
             raise ValueError("residual_norm: gate must be [C], or x's shape with trailing dims before the "
                              "last of size 1 ([B, 1, C], [B, N, C])")
-    _device_of(x, y, gate, weight, bias, post_weight, post_bias, what="residual_norm")
+    _one_device(x, y, gate, weight, bias, post_weight, post_bias, what="residual_norm")
+
+
+def _leads(part, full) -> bool:
+    """Whether `part` is `full` with some trailing dims of size 1."""
+    n = len(part)
+    if n != len(full):
+        return False
+    while n and part[n - 1] == 1:
+        n -= 1
+    return part[:n] == full[:n]
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = None,
@@ -792,11 +850,14 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor]
     C % 8 == 0, C <= 8192.  Differentiable once in x, y, gate and the norm
     parameters; column sums run in a fixed order."""
     _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind, post_kind)
-    args = (x, y, gate, weight, bias, post_weight, post_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        out = _ResidualNorm.apply(*args, float(eps), kind, post_kind, float(post_eps))
-        return out if kind is not None else (out, None)
-    return _residual_norm_launch(*args, float(eps), kind, post_kind, float(post_eps), False)[:2]
+    if torch.is_grad_enabled():
+        for t in (x, y, gate, weight, bias, post_weight, post_bias):
+            if t is not None and t.requires_grad:
+                out = _ResidualNorm.apply(x, y, gate, weight, bias, post_weight, post_bias, eps, kind, post_kind,
+                                          post_eps)
+                return out if kind is not None else (out, None)
+    return _residual_norm_launch(x, y, gate, weight, bias, post_weight, post_bias, eps, kind, post_kind, post_eps,
+                                 False)[:2]
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_norm, k_norm, positions: Optional[torch.Tensor],

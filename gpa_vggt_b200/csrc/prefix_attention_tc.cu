@@ -9,10 +9,9 @@
 //              bits) that one more K=16 step adds to the scores, -inf for keys
 //              that are out.
 //   warps 1-2  MMA issuers, one per row tile: S = Q K^T (+ bias), O += P V with P
-//              from TMEM.
-//   warp 3     zeroes the K and V rows of keys that are out (past a request's
-//              length, or -inf in the bias), whose memory may hold anything, and
-//              passes the tile on.
+//              from TMEM.  Before a tile's first product they zero the K and V
+//              rows of keys that are out (past a request's length, or -inf in the
+//              bias), whose memory may hold anything.
 //   warps 4-11 two softmax warpgroups, a thread per row: S from TMEM, running
 //              maximum that moves only by more than 2^8, P back as bf16.
 // At head_dim 64 S, P and O of both tiles fit TMEM side by side and S(j+1) runs
@@ -26,7 +25,11 @@ namespace prefix {
 constexpr int TC_THREADS = 384;
 constexpr int TM = 128;   // rows and keys per tile
 constexpr int XTILE = TM * 16 * 2;
-constexpr float kBiasLimit = 1.0e30f;   // finite biases end here (score units)
+// Finite biases end here (log2 units).  A row of nothing but the type's lowest
+// value spreads evenly: scores up to 64 vanish beside 2^30, and c*x - c*m, off by
+// the rounding of c*m (at most 64, the same for all of a row's keys), stays inside
+// the exponent's range.
+constexpr float kBiasLimit = 1073741824.f;
 constexpr int TC_REGS = 168, TC_LOW = 80, TC_HIGH = 208;
 static_assert(TC_LOW * 128 + TC_HIGH * 256 <= TC_REGS * TC_THREADS, "register split");
 
@@ -45,7 +48,7 @@ struct TcSmem {
   static constexpr int BARS = MASK + STAGES * 16;
   static constexpr int TOTAL = BARS + 256;
   static constexpr int ALLOC = TOTAL + 1024;
-  static_assert((1 + 6 * STAGES + 8) * 8 + 8 <= 256, "barrier area");
+  static_assert((1 + 4 * STAGES + 8) * 8 + 8 <= 256, "barrier area");
   static_assert(ALLOC <= 232448, "shared memory per CTA");
 };
 
@@ -160,9 +163,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
   uint64_t* k_full = q_full + 1;       // TMA landed
   uint64_t* v_full = k_full + ST;
-  uint64_t* k_ok = v_full + ST;        // and passed on by warp 3
-  uint64_t* v_ok = k_ok + ST;
-  uint64_t* k_empty = v_ok + ST;
+  uint64_t* k_empty = v_full + ST;
   uint64_t* v_empty = k_empty + ST;
   uint64_t* s_full = v_empty + ST;     // 2
   uint64_t* s_empty = s_full + 2;      // 2
@@ -177,8 +178,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       bar_init(&k_full[s], 1);
       bar_init(&v_full[s], 1);
-      bar_init(&k_ok[s], 1);
-      bar_init(&v_ok[s], 1);
       bar_init(&k_empty[s], active);   // one arrival per stream that reads the tile
       bar_init(&v_empty[s], active);
     }
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int row = lane; row < TM; row += 32)   // 1, 1, 1, 0, ...
         *reinterpret_cast<uint2*>(smem + SM::ONES + xtile_off(row, 0)) = make_uint2(0x3F803F80u, 0x3F80u);
       const float* brow = p.bias ? p.bias + kh * p.bias_sh : nullptr;
-      const float inv_scale = 1.0f / p.scale;
+      const float inv_scale = 1.0f / p.scale, most = kBiasLimit / p.scale_log2;
       float braw[4];
       auto load_bias = [&](int j) {   // raw bias of a tile, one tile ahead of its use
 #pragma unroll
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           for (int i = 0; i < 4; ++i) {
             const int row = i * 32 + lane;
             const bool in = row < t.valid && braw[i] > -INFINITY;   // NaN takes a key out too
-            const float beta = in ? fminf(fmaxf(braw[i] * inv_scale, -kBiasLimit), kBiasLimit) : -INFINITY;
+            const float beta = in ? fminf(fmaxf(braw[i] * inv_scale, -most), most) : -INFINITY;
             const __nv_bfloat16 hi = __float2bfloat16_rn(beta);
             float rest = in ? beta - __bfloat162float(hi) : 0.f;
             const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
@@ -284,38 +283,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         drain_bar(q_full, 0, t0);
         for (int j = max(0, issued_k - ST); j < issued_k; ++j) drain_bar(&k_full[j % ST], (j / ST) & 1, t0);
         for (int j = max(0, issued_v - ST); j < issued_v; ++j) drain_bar(&v_full[j % ST], (j / ST) & 1, t0);
-      }
-    } else if (warp == 3) {
-      // ------------------------------ gate of the rings ------------------------------
-      for (int j = 0; j < nk; ++j) {
-        const int s = j % ST;
-        const uint32_t ph = (j / ST) & 1;
-        const Tile t = tile_of(j);
-        const bool look = t.own ? t.valid < TM : p.bias != nullptr;
-        uint32_t m[4] = {0u, 0u, 0u, 0u};
-        auto zero_rows = [&](uint8_t* base) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            for (uint32_t left = m[i]; left; left &= left - 1) {
-              const int row = i * 32 + __ffs(left) - 1;
-              if (lane < 8 * SM::HALVES)
-                *reinterpret_cast<uint4*>(base + (lane >> 3) * SM::HALF + row * 128 + (lane & 7) * 16) =
-                    make_uint4(0u, 0u, 0u, 0u);
-            }
-          fence_async_smem();
-          __syncwarp();
-        };
-        if (!wait(&k_full[s], ph)) break;
-        if (look) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m[i] = *(reinterpret_cast<volatile uint32_t*>(smem + SM::MASK + s * 16) + i);
-        }
-        const bool any = (m[0] | m[1] | m[2] | m[3]) != 0;
-        if (any) zero_rows(smem + SM::K + s * SM::TILE);
-        if (lane == 0) bar_arrive(&k_ok[s]);
-        if (!wait(&v_full[s], ph)) break;
-        if (any) zero_rows(smem + SM::V + s * SM::TILE);
-        if (lane == 0) bar_arrive(&v_ok[s]);
       }
     } else if (warp - 1 < streams) {
       // ------------------------------ MMA issuers ------------------------------
@@ -360,29 +327,53 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         __syncwarp();
       };
-      auto wait_tile = [&](uint64_t* bar, int j) { return wait(&bar[key_tile(j) % ST], key_tile(j) / ST); };
-      bool okw = wait(q_full, 0) && wait_tile(k_ok, 0);
-      if (okw) {
-        tc_fence_after();
-        issue_s(0);
-      }
-      for (int j = 0; okw && j < n; ++j) {
-        if (D == 64 && j + 1 < n) {
-          okw = wait(&s_empty[t], j) && wait_tile(k_ok, j + 1);
-          if (!okw) break;
-          tc_fence_after();
-          issue_s(j + 1);
+      // The rows to zero of a key tile, read once its K has landed (the producer
+      // reuses the words before its V is used).
+      auto rows_out = [&](int j) {
+        const Tile kt = tile_of(key_tile(j));
+        return (kt.own ? kt.valid < TM : p.bias != nullptr)
+                   ? *reinterpret_cast<const uint4*>(smem + SM::MASK + (key_tile(j) % ST) * 16)
+                   : make_uint4(0u, 0u, 0u, 0u);
+      };
+      // Where both issuers read a tile, the second writes the same zeros.
+      auto zero_rows = [&](const uint4& m, int base, int j) {
+        if (!(m.x | m.y | m.z | m.w)) return;
+        uint8_t* tile = smem + base + (key_tile(j) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
+        for (int row = 0; row < TM; ++row) {
+          const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
+          if ((word >> (row & 31) & 1) && lane < 8 * SM::HALVES)
+            *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
         }
-        okw = wait(&p_full[t], j) && wait_tile(v_ok, j);
+        fence_async_smem();
+        __syncwarp();
+      };
+      auto wait_tile = [&](uint64_t* bar, int j) { return wait(&bar[key_tile(j) % ST], key_tile(j) / ST); };
+      uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
+      auto scores = [&](int j) {   // once K has landed
+        tc_fence_after();
+        out_next = rows_out(j);
+        zero_rows(out_next, SM::K, j);
+        issue_s(j);
+      };
+      bool okw = wait(q_full, 0) && wait_tile(k_full, 0);
+      if (okw) scores(0);
+      for (int j = 0; okw && j < n; ++j) {
+        out_now = out_next;
+        if (D == 64 && j + 1 < n) {
+          okw = wait(&s_empty[t], j) && wait_tile(k_full, j + 1);
+          if (!okw) break;
+          scores(j + 1);
+        }
+        okw = wait(&p_full[t], j) && wait_tile(v_full, j);
         if (!okw) break;
         tc_fence_after();
+        zero_rows(out_now, SM::V, j);
         issue_o(j);
         if (D == 128 && j + 1 < n) {
           // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
-          okw = wait_tile(k_ok, j + 1) && wait(&o_done[t], j);
+          okw = wait_tile(k_full, j + 1) && wait(&o_done[t], j);
           if (!okw) break;
-          tc_fence_after();
-          issue_s(j + 1);
+          scores(j + 1);
         }
       }
     }
@@ -398,8 +389,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const Row row = row_of(halves ? 0 : t, quad * 32 + lane);
       const bool idle = !__any_sync(0xffffffffu, row.live);   // a warp without rows only keeps the barriers going
       // own keys that this row sees end here
-      const int limit = p.causal && !tc.fold ? len - qlen + row.m + 1 : 0x7fffffff;
-      float m_raw = -INFINITY, l = 0.f;   // running maximum (score units), row sum
+      const bool ordered = p.causal && !tc.fold;
+      const int limit = ordered ? len - qlen + row.m + 1 : 0x7fffffff;
+      constexpr float kNoMax = -3.0e38f;   // no key yet
+      float m_raw = kNoMax, l = 0.f;       // running maximum (score units), row sum
+      float neg_mc = 0.f;                  // -c2 * m_raw
       const float c2 = p.scale_log2;
       bool okw = true;
       auto quarter = [&](float* xq, float neg_mc, float* acc, uint32_t* pk) {
@@ -416,18 +410,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           for (int i = 0; i < 4; ++i) pk[g * 4 + i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
         }
       };
-      for (int j = 0; j < n; ++j) {
-        if (!wait(&s_full[t], j)) { okw = false; break; }
-        tc_fence_after();
-        if (idle) {
+      if (idle) {
+        for (int j = 0; j < n; ++j) {
           // S(j+1) may be there before the other warps' P(j): no second arrival in one phase
-          if (j > 0 && !wait(&p_full[t], j - 1)) { okw = false; break; }
+          okw = wait(&s_full[t], j) && (j == 0 || wait(&p_full[t], j - 1));
+          if (!okw) break;
           if (lane == 0) {
             if (D == 64) bar_arrive(&s_empty[t]);
             bar_arrive(&p_full[t]);
           }
-          continue;
         }
+      }
+      for (int j = idle ? n : 0; j < n; ++j) {
+        if (!wait(&s_full[t], j)) { okw = false; break; }
+        tc_fence_after();
         float x[TM];
 #pragma unroll
         for (int c = 0; c < TM / 32; ++c) tmem_ld32f(tS + c * 32, x + c * 32);
@@ -435,12 +431,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
-        const Tile kt = tile_of(halves ? 2 * j + t : j);
-        if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {   // keys ahead of this row
-          const int end = limit - kt.key0;
+        if (ordered) {   // keys ahead of this row
+          const Tile kt = tile_of(halves ? 2 * j + t : j);
+          if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {
+            const int end = limit - kt.key0;
 #pragma unroll
-          for (int c = 0; c < TM; ++c)
-            if (c >= end) x[c] = -INFINITY;
+            for (int c = 0; c < TM; ++c)
+              if (c >= end) x[c] = -INFINITY;
+          }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -449,22 +447,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           mx[c & 3] = max3_nan(mx[c & 3], x[4 * c + 2], x[4 * c + 3]);
         }
         const float mt = max3_nan(max3_nan(mx[0], mx[0], mx[1]), mx[2], mx[3]);
-        if (!(mt < INFINITY)) l = NAN;   // a NaN or an infinite score: the row is NaN (the polynomial would lose it)
         float alpha = 1.f;
-        const bool moved = (mt - m_raw) * c2 > 8.0f;   // also from -inf (both -inf: no)
-        if (moved) {
-          alpha = fast_exp2((m_raw - mt) * c2);
-          l *= alpha;
-          m_raw = mt;
-        }
-        float neg_mc = m_raw > -INFINITY ? -m_raw * c2 : 0.f;
-        // c*x - c*m carries the rounding of c*m, which a row of the lowest biases
-        // makes larger than the exponent's range: there the difference comes first
-        if (__any_sync(0xffffffffu, fabsf(neg_mc) > 1048576.f)) {
-          const float m = m_raw > -INFINITY ? m_raw : 0.f;
-#pragma unroll
-          for (int c = 0; c < TM; ++c) x[c] -= m;
-          neg_mc = 0.f;
+        // the maximum moves: also the first time, and for a NaN (never for a row without keys)
+        const bool moved = row.live && !((mt - m_raw) * c2 <= 8.0f);
+        const bool any_moved = __any_sync(0xffffffffu, moved);
+        if (any_moved) {
+          if (moved) {
+            alpha = fast_exp2((m_raw - mt) * c2);
+            l = mt < INFINITY ? l * alpha : NAN;   // a NaN or infinite score: the row is NaN (the polynomial would lose it)
+            m_raw = mt < INFINITY ? mt : 0.f;
+            neg_mc = -m_raw * c2;
+          }
         }
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         uint32_t pk[4][16];
@@ -486,7 +479,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         if (!okw) break;
         l += ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
-        if (j > 0 && __any_sync(0xffffffffu, moved)) {
+        if (j > 0 && any_moved) {
           uint32_t ov[32];
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
@@ -529,13 +522,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         float f0 = 1.f;
         if (halves) {
           const float m1 = xml[0], m = fmaxf(m_raw, m1);
-          const bool any = m > -INFINITY;   // else the sums hold the polynomial's 2^-126, or a NaN
-          f0 = any ? fast_exp2((m_raw - m) * c2) : 1.f;
-          f1 = any ? fast_exp2((m1 - m) * c2) : 1.f;
+          f0 = fast_exp2((m_raw - m) * c2);
+          f1 = fast_exp2((m1 - m) * c2);
           l = l * f0 + xml[1] * f1;
           m_raw = m;
         }
-        const bool some = m_raw > -INFINITY || l != l;
+        const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
         const float inv = some ? 1.0f / l : 0.f;
         const int64_t at = split * p.rows + row_index(p, row);
         __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
@@ -567,7 +559,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         if (row.live) {
           if (partial)
-            p.ws_ml[at] = make_float2(m_raw * c2, some ? l : 0.f);
+            p.ws_ml[at] = some ? make_float2(m_raw * c2, l) : make_float2(-INFINITY, 0.f);
           else if (p.lse)
             p.lse[row.r * p.lse_sr + row.h * p.lse_sh + row.m] = some ? m_raw * c2 + log2f(l) : -INFINITY;
         }

@@ -24,6 +24,8 @@ namespace prefix {
 constexpr int BN = 64;         // keys per tile
 constexpr int THREADS = 128;
 constexpr int kSlotTiles = 4;  // at least this many tiles per chunk
+constexpr int kSms = 148;
+constexpr int kLeastSpan = 4;  // at least this many steps per CTA of the tensor-core kernel
 
 template <int D>
 struct Cfg {
@@ -372,6 +374,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const int slots = p.s1 + p.s2;
   const float2* mlr = p.ws_ml + row;
   const float2 first = lane < slots ? mlr[lane * p.rows] : make_float2(-INFINITY, 0.f);
+  if (__shfl_sync(0xffffffffu, first.y, 0) == kWritten) return;   // by the tensor-core kernel
   float mx = first.x;
   for (int s = lane + 32; s < slots; s += 32) mx = fmaxf(mx, mlr[s * p.rows].x);
 #pragma unroll
@@ -463,30 +466,10 @@ struct Plan {
   int64_t items, rows;
   TcPlan tc;
   int64_t slots() const { return s1 + s2; }
-  bool joins() const { return !(tc_run && !rows_run && s1 == 1); }   // else outputs are written at once
-  int64_t bytes(int head_dim) const { return joins() ? slots() * rows * (head_dim + 2) * 4 : 0; }
+  int64_t bytes(int head_dim) const { return slots() * rows * (head_dim + 2) * 4; }
 };
 
 static int warps_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-
-// Chunks of key tiles per item of the tensor-core kernel: whole waves of 148
-// CTAs, each chunk with a few tiles' worth of start-up and end, against the
-// partial outputs that every chunk writes and the join reads.
-static int tc_splits(int64_t items, int64_t tiles, int64_t rows, int head_dim) {
-  const double tile_us = head_dim == 64 ? 1.5 : 2.2;
-  int best = 1;
-  double least = 0;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const double waves = (double)((items * s + 147) / 148);
-    double us = waves * ((double)((tiles + s - 1) / s) + 3) * tile_us;
-    if (s > 1) us += 4 + (double)s * rows * head_dim * 8 / 4e6;
-    if (s == 1 || us < least) {
-      least = us;
-      best = s;
-    }
-  }
-  return best;
-}
 
 // joint, fold: whether the tensor-core kernel can take the call in that form.
 static Plan make_plan(int requests, int queries, int heads, int kv_heads, int head_dim, int prefix, int cache,
@@ -503,12 +486,18 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
     p.tc.fold = fold;
     p.tc.tokens = fold ? requests * queries : queries;
     p.tc.per_tile = 128 / group;
-    p.tc.pairs = (p.tc.tokens + 2 * p.tc.per_tile - 1) / (2 * p.tc.per_tile);
-    const int64_t tiles = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
-    const int64_t items = (int64_t)p.tc.pairs * kv_heads * (fold ? 1 : requests);
-    const int s = tc_splits(items, tiles, p.rows, head_dim);
-    p.tc.per = (int)((tiles + s - 1) / s);
-    p.s1 = p.tc.splits = (int)((tiles + p.tc.per - 1) / p.tc.per);
+    // The steps of all items at full lengths (the kernel counts the real ones),
+    // and what a CTA gets of them.  An item is cut where a span ends: at most
+    // steps / span + 2 parts; twice the steps / span leaves room for spans that
+    // shorter lengths make shorter.
+    const int64_t tiles = (p.tc.tokens + p.tc.per_tile - 1) / p.tc.per_tile;
+    const int64_t steps = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
+    const int64_t total = ((tiles >> 1) * steps + (tiles & 1 ? (steps + 1) / 2 : 0)) * kv_heads * (fold ? 1 : requests);
+    const int64_t span = std::max<int64_t>((total + kSms - 1) / kSms, kLeastSpan);
+    const int64_t cuts = std::min<int64_t>(2 * ((steps + span - 1) / span), std::max<int64_t>(steps / kLeastSpan, 1));
+    p.tc.least = (int)std::max<int64_t>((steps + cuts - 1) / cuts, kLeastSpan);
+    p.tc.ctas = (int)std::min<int64_t>(kSms, (total + kLeastSpan - 1) / kLeastSpan);
+    p.s1 = (int)((steps + p.tc.least - 1) / p.tc.least) + 1;
   }
   if (p.rows_run) {
     const int64_t t1 = p.tc_run ? 0 : (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
@@ -551,7 +540,7 @@ static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
       default: rc = launch_rows<D, 4, 4>(p, plan.items, st); break;
     }
   }
-  if (rc || !plan.joins()) return rc;
+  if (rc) return rc;
   return launch_join<D>(p, st);
 }
 
@@ -636,7 +625,7 @@ extern "C" int gpa_attention_shared_prefix(
   const prefix::Plan plan =
       prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len,
                         prefix::tc_takes(p, head_dim, false), prefix::tc_takes(p, head_dim, true));
-  if (plan.items >= (1ll << 31) || (int64_t)plan.tc.pairs * plan.tc.splits * kv_heads * requests >= (1ll << 31))
+  if (plan.items >= (1ll << 31))
     return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
   const int64_t bytes = plan.bytes(head_dim);
   if (bytes && (!workspace || !aligned16(workspace) || workspace_bytes < bytes))

@@ -45,15 +45,17 @@ __device__ __forceinline__ int query_count(const Params& p, int r) {
   return p.q_len ? min(max(__ldg(p.q_len + r), 0), p.queries) : p.queries;
 }
 
+// What the sum of a row's first partial output holds when its output is written.
+constexpr float kWritten = -1.0f;
+
 // The tensor-core kernel's share of a call: 2 x 128-row tiles over the prefix
 // and, unless `fold`, each request's own keys.
 struct TcPlan {
   int fold;      // rows run through all requests (prefix only), else within one request
   int tokens;    // tokens a tile's rows may come from: requests * queries (fold) or queries
   int per_tile;  // tokens of a 128-row tile
-  int pairs;     // tile pairs over the tokens
-  int splits;    // chunks over the key tiles
-  int per;       // key tiles per chunk
+  int ctas;      // each takes a span of the key-tile steps
+  int least;     // of at least so many: no item is cut into more than s1 parts
 };
 // Whether the kernel can take the call's strides and scale.
 bool tc_takes(const Params& p, int head_dim, bool fold);

@@ -1,22 +1,30 @@
 // Attention over a shared prefix and own keys for many query rows, on the
 // 5th-generation tensor cores (see prefix_attention.cu for the call).
 //
-// One CTA takes two 128-row tiles of one key/value head and one chunk of the key
-// tiles: the prefix's, then the request's own ones, in one online softmax.  384
-// threads:
-//   warp 0     TMA producer: Q once, then K and V tiles of 128 keys through a
-//              ring each; writes a tile's bias / scale as three bf16 terms (24
-//              bits) that one more K=16 step adds to the scores, -inf for keys
-//              that are out.
-//   warps 1-2  MMA issuers, one per row tile: S = Q K^T (+ bias), O += P V with P
-//              from TMEM.  Before a tile's first product they zero the K and V
-//              rows of keys that are out (past a request's length, or -inf in the
-//              bias), whose memory may hold anything.
-//   warps 4-11 two softmax warpgroups, a thread per row: S from TMEM, running
-//              maximum that moves only by more than 2^8, P back as bf16.
-// At head_dim 64 S, P and O of both tiles fit TMEM side by side and S(j+1) runs
+// An item is a pair of 128-row tiles of one key/value head and all of its key
+// tiles: the prefix's, then the request's own ones, in one online softmax.  One
+// CTA per SM; the items' key tiles, laid end to end, are dealt out in equal spans,
+// so that a CTA may begin and end inside an item (its part is joined later) and
+// no wave is left half empty: the lengths on the device set the spans.  A pair of
+// which only one tile has rows runs it over the even and the odd key tiles at
+// once instead.  384 threads:
+//   warp 0     TMA producer: Q, then K and V tiles of 128 keys through a ring
+//              each, on into the next item; writes a tile's bias / scale as three
+//              bf16 terms (24 bits) that one more K=16 step adds to the scores,
+//              -inf for keys that are out.
+//   warps 1-2  MMA issuers, one per stream (row tile, or half of the key tiles):
+//              S = Q K^T (+ bias), O += P V with P from TMEM.  Before a tile's
+//              first product they zero the K and V rows of keys that are out (past
+//              a request's length, or -inf in the bias), whose memory may hold
+//              anything.
+//   warp 3     works out the CTA's pieces ahead of the others and hands them on in
+//              a small ring.
+//   warps 4-11 two softmax warpgroups, one per stream, a thread per row: S from
+//              TMEM, running maximum that moves only by more than 2^8, P back as
+//              bf16.
+// At head_dim 64 S, P and O of both streams fit TMEM side by side and S(j+1) runs
 // during the softmax of S(j).  At 128 P(j) takes the columns of S(j), and S(j+1)
-// waits for O += P(j) V; the other tile's softmax runs meanwhile.
+// waits for O += P(j) V; the other stream's softmax runs meanwhile.
 #include "prefix_attention.cuh"
 
 namespace gpa {
@@ -33,6 +41,8 @@ constexpr float kBiasLimit = 1073741824.f;
 constexpr int TC_REGS = 168, TC_LOW = 80, TC_HIGH = 208;
 static_assert(TC_LOW * 128 + TC_HIGH * 256 <= TC_REGS * TC_THREADS, "register split");
 
+constexpr int RING = 4;   // pieces handed on ahead
+
 template <int D>
 struct TcSmem {
   static constexpr int HALVES = D / 64;          // a row is HALVES swizzled rows of 128 bytes
@@ -45,10 +55,11 @@ struct TcSmem {
   static constexpr int ONES = V + STAGES * TILE;
   static constexpr int BETA = ONES + XTILE;
   static constexpr int MASK = BETA + STAGES * XTILE;   // 4 words per stage
-  static constexpr int BARS = MASK + STAGES * 16;
-  static constexpr int TOTAL = BARS + 256;
+  static constexpr int ML = MASK + STAGES * 16;        // the second stream's maxima and sums
+  static constexpr int BARS = ML + TM * 8;
+  static constexpr int TOTAL = BARS + 384;
   static constexpr int ALLOC = TOTAL + 1024;
-  static_assert((1 + 4 * STAGES + 8) * 8 + 8 <= 256, "barrier area");
+  static_assert((4 + 4 * STAGES + 8 + 2 * RING) * 8 + 8 <= 384, "barrier area");
   static_assert(ALLOC <= 232448, "shared memory per CTA");
 };
 
@@ -69,9 +80,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// The two softmax warpgroups.
-__device__ __forceinline__ void named_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 // 2 of 8 exponentials on the FMA pipe, the rest on MUFU
 __device__ __forceinline__ void exp8(const float* x, float* e) {
 #pragma unroll
@@ -79,7 +87,74 @@ __device__ __forceinline__ void exp8(const float* x, float* e) {
   exp2_poly2<3>(x[6], x[7], e[6], e[7]);
 }
 
-template <int D>
+// The order of work: requests, their key heads, the head's row-tile pairs, a
+// pair's steps.  A step is one key tile for two row tiles or two for one.
+struct Load {
+  int pairs2;      // pairs with two row tiles
+  bool single;     // and one with one
+  int nk;          // key tiles (none at all counts as one, to write the empty rows)
+  int64_t head;    // steps of one key head
+};
+__device__ __forceinline__ Load load_of(const Params& p, const TcPlan& tc, int r) {
+  Load w;
+  const int tokens = tc.fold ? tc.tokens : query_count(p, r);
+  const int tiles = (tokens + tc.per_tile - 1) / tc.per_tile;
+  w.pairs2 = tiles >> 1;
+  w.single = tiles & 1;
+  w.nk = max(1, (p.prefix + TM - 1) / TM + (tc.fold ? 0 : (own_length(p, r) + TM - 1) / TM));
+  w.head = (int64_t)w.pairs2 * w.nk + (w.single ? (w.nk + 1) >> 1 : 0);
+  return w;
+}
+
+// A CTA's share of one item.
+struct Piece {
+  int req, kh, tok0, tok_end;
+  int active;        // row tiles with rows: 1 or 2
+  int len, qlen;
+  int j0, nk;        // key tiles (nk may be 0: nothing to see here)
+  int slot;          // which partial output
+  bool first, last;  // holds the item's first, last step
+};
+struct Walk {
+  int64_t pos, end, span;   // this CTA's steps
+  int req;
+  int64_t req0;             // first step of the request
+};
+__device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Walk& w, Piece& c) {
+  if (w.pos >= w.end) return false;
+  Load ld = load_of(p, tc, w.req);
+  while (w.pos - w.req0 >= ld.head * p.kv_heads) {
+    w.req0 += ld.head * p.kv_heads;
+    ld = load_of(p, tc, ++w.req);
+  }
+  const int64_t x = w.pos - w.req0;
+  c.req = w.req;
+  c.kh = (int)(x / ld.head);
+  const int64_t y = x - c.kh * ld.head;
+  const int pair = (int)min(y / ld.nk, (int64_t)ld.pairs2);
+  const int a = (int)(y - (int64_t)pair * ld.nk);
+  c.active = pair < ld.pairs2 ? 2 : 1;
+  const int steps = c.active == 2 ? ld.nk : (ld.nk + 1) >> 1;
+  const int b = (int)min((int64_t)steps, a + (w.end - w.pos));
+  c.tok0 = pair * 2 * tc.per_tile;
+  c.qlen = tc.fold ? p.queries : query_count(p, c.req);
+  c.tok_end = tc.fold ? tc.tokens : c.qlen;
+  c.len = tc.fold ? 0 : own_length(p, c.req);
+  // with an order, no row of this pair sees an own key from here on
+  const int own_end =
+      p.causal ? min(c.len, max(0, c.len - c.qlen + min(c.tok0 + 2 * tc.per_tile, c.qlen))) : c.len;
+  const int tiles = (p.prefix + TM - 1) / TM + (own_end + TM - 1) / TM, each = 3 - c.active;
+  c.j0 = a * each;
+  c.nk = max(0, min(tiles, b * each) - c.j0);
+  c.first = a == 0;
+  c.last = b == steps;
+  c.slot = (int)(blockIdx.x - (w.pos - a) / w.span);
+  w.pos += b - a;
+  return true;
+}
+
+// CAUSAL: own keys in order (a kernel of its own: the mask costs the others registers).
+template <int D, bool CAUSAL>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kp,
               const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_ko,
@@ -87,81 +162,56 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   using SM = TcSmem<D>;
   constexpr int ST = SM::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ int64_t warp_steps[TC_THREADS / 32];
+  __shared__ int64_t start_req0;
+  __shared__ int start_req;
+  __shared__ Piece ring[RING];
   asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
+  const int warp = warp_id(), lane = lane_id();
 
-  // the item: row tiles fastest, then requests, so that CTAs running together
-  // read the same keys of the prefix
-  int it = blockIdx.x;
-  const int pair = it % tc.pairs;
-  it /= tc.pairs;
-  const int nreq = tc.fold ? 1 : p.requests;
-  const int req = it % nreq;
-  it /= nreq;
-  const int split = it % tc.splits;
-  const int kh = it / tc.splits;
-  const int tok0 = pair * 2 * tc.per_tile;
-  const int qlen = tc.fold ? p.queries : query_count(p, req);
-  const int tok_end = tc.fold ? tc.tokens : qlen;
-  if (tok0 >= tok_end) return;   // padding only: nothing to write
-  const int active = tok0 + tc.per_tile < tok_end ? 2 : 1;   // row tiles with rows
-  const int len = tc.fold ? 0 : own_length(p, req);
-  // with an order, no row of this item sees an own key from here on
-  const int own_end = p.causal ? min(len, max(0, len - qlen + min(tok0 + 2 * tc.per_tile, qlen))) : len;
-  const int tp = (p.prefix + TM - 1) / TM;
-  const int j0 = split * tc.per;
-  const int nk = max(0, min(tp + (own_end + TM - 1) / TM, j0 + tc.per) - j0);
-  // Two streams of work for the issuers and softmax warpgroups: the two row
-  // tiles over the same key tiles, or, where only one has rows, that one over the
-  // even and the odd key tiles (joined at the end).
-  const bool halves = active == 1 && nk > 1;
-  const int streams = nk > 1 ? 2 : active;
-  const bool partial = p.s1 + p.s2 > 1;
-  auto row_of = [&](int t, int i) {
-    Row w;
-    const int tl = i / p.group;
-    const int tok = tok0 + t * tc.per_tile + tl;
-    w.h = kh * p.group + (i - tl * p.group);
-    w.live = tl < tc.per_tile && tok < tok_end;
-    w.r = req;
-    w.m = tok;
-    if (tc.fold) {
-      w.r = tok / p.queries;
-      w.m = tok - w.r * p.queries;
-      if (w.live && p.q_len) w.live = w.m < __ldg(p.q_len + w.r);
+  // All steps, this CTA's span of them, and the request that it starts in: each
+  // thread adds up a run of requests.
+  Walk walk;
+  {
+    const int nreq = tc.fold ? 1 : p.requests;
+    const int run = (nreq + TC_THREADS - 1) / TC_THREADS;
+    const int r0 = threadIdx.x * run, r1 = min(nreq, r0 + run);
+    int64_t mine = 0;
+    for (int r = r0; r < r1; ++r) mine += load_of(p, tc, r).head * p.kv_heads;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
     }
-    return w;
-  };
-  if (nk == 0) {   // no keys in this chunk
-    for (int i = threadIdx.x; i < 2 * TM; i += TC_THREADS) {
-      const Row w = row_of(i / TM, i % TM);
-      if (!w.live) continue;
-      if (partial) {
-        p.ws_ml[split * p.rows + row_index(p, w)] = make_float2(-INFINITY, 0.f);
-      } else {
-        uint4* o = reinterpret_cast<uint4*>(p.o + w.r * p.o_sr + w.h * p.o_sh + w.m * p.o_sm);
-        for (int u = 0; u < D / 8; ++u) o[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (p.lse) p.lse[w.r * p.lse_sr + w.h * p.lse_sh + w.m] = -INFINITY;
+    if (lane == 31) warp_steps[warp] = upto;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int i = 0; i < TC_THREADS / 32; ++i) {
+      if (i < warp) before += warp_steps[i];
+      total += warp_steps[i];
+    }
+    walk.span = max((total + gridDim.x - 1) / gridDim.x, (int64_t)tc.least);
+    walk.pos = blockIdx.x * walk.span;
+    walk.end = min(total, walk.pos + walk.span);
+    if (walk.pos >= total) return;   // the whole CTA
+    int64_t at = before + upto - mine;
+    if (walk.pos >= at && walk.pos < at + mine) {
+      int r = r0;
+      for (;; ++r) {
+        const int64_t n = load_of(p, tc, r).head * p.kv_heads;
+        if (walk.pos < at + n) break;
+        at += n;
       }
+      start_req = r;
+      start_req0 = at;
     }
-    return;
   }
-  // key tile j (of this chunk): the prefix's or an own one
-  struct Tile {
-    bool own;
-    int key0, valid;   // keys of the tile that exist
-  };
-  auto tile_of = [&](int j) {
-    Tile t;
-    t.own = j0 + j >= tp;
-    t.key0 = (t.own ? j0 + j - tp : j0 + j) * TM;
-    t.valid = min(TM, (t.own ? len : p.prefix) - t.key0);
-    return t;
-  };
-  auto has_beta = [&](const Tile& t) { return t.valid < TM || (!t.own && p.bias != nullptr); };
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
-  uint64_t* k_full = q_full + 1;       // TMA landed
+  uint64_t* q_empty = q_full + 1;      // both streams' score products of the item are done
+  uint64_t* k_full = q_empty + 1;
   uint64_t* v_full = k_full + ST;
   uint64_t* k_empty = v_full + ST;
   uint64_t* v_empty = k_empty + ST;
@@ -169,17 +219,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* s_empty = s_full + 2;      // 2
   uint64_t* p_full = s_empty + 2;      // 2
   uint64_t* o_done = p_full + 2;       // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* half_there = o_done + 2;   // the second stream's half is complete
+  uint64_t* half_read = half_there + 1;
+  uint64_t* piece_full = half_read + 1;      // RING
+  uint64_t* piece_empty = piece_full + RING;   // RING
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_empty + RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = warp_id(), lane = lane_id();
 
+  // Every barrier's phases run on through the CTA's pieces: per role, `g` counts
+  // the key tiles of all pieces so far, `c` those of one stream, `i` the pieces
+  // that have key tiles.
   if (threadIdx.x == 0) {
     bar_init(q_full, 1);
+    bar_init(q_empty, 2);
     for (int s = 0; s < ST; ++s) {
       bar_init(&k_full[s], 1);
       bar_init(&v_full[s], 1);
-      bar_init(&k_empty[s], active);   // one arrival per stream that reads the tile
-      bar_init(&v_empty[s], active);
+      bar_init(&k_empty[s], 2);   // one arrival per row tile, or two by the one stream that reads the tile
+      bar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       bar_init(&s_full[t], 1);
@@ -187,6 +244,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       bar_init(&p_full[t], 4);
       bar_init(&o_done[t], 1);
     }
+    for (int s = 0; s < RING; ++s) {
+      bar_init(&piece_full[s], 1);
+      bar_init(&piece_empty[s], 11);   // producer, issuers, softmax warps
+    }
+    bar_init(half_there, 4);
+    bar_init(half_read, 4);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -198,10 +261,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {   // the whole warp, bounded
-    return __all_sync(0xffffffffu, wait_bar(bar, parity & 1, abort_flag, p.status, kDevTimeout)) != 0;
+  const int tp = (p.prefix + TM - 1) / TM;
+  auto wait = [&](uint64_t* bar, uint32_t phase) {   // the whole warp, bounded
+    return __all_sync(0xffffffffu, wait_bar(bar, phase & 1, abort_flag, p.status, kDevTimeout)) != 0;
   };
-  // TMEM columns of a row tile
+  // The next piece of the ring (`turn` counts them) into c, or false at the end;
+  // done() gives its place back.
+  auto next = [&](Piece& c, uint32_t turn, bool& okw) {
+    okw = wait(&piece_full[turn % RING], turn / RING);
+    if (!okw) return false;
+    c = ring[turn % RING];
+    return c.req >= 0;
+  };
+  auto done = [&](uint32_t turn) {
+    __syncwarp();
+    if (lane == 0) bar_arrive(&piece_empty[turn % RING]);
+  };
+  // key tile j of a piece: the prefix's or an own one
+  struct Tile {
+    bool own;
+    int key0, valid;   // keys of the tile that exist
+  };
+  auto tile_of = [&](const Piece& c, int j) {
+    Tile t;
+    t.own = c.j0 + j >= tp;
+    t.key0 = (t.own ? c.j0 + j - tp : c.j0 + j) * TM;
+    t.valid = min(TM, (t.own ? c.len : p.prefix) - t.key0);
+    return t;
+  };
+  auto has_beta = [&](const Tile& t) { return t.valid < TM || (!t.own && p.bias != nullptr); };
+  // key tiles of stream t, and which they are
+  auto tiles_of = [](const Piece& c, int t) { return c.active == 2 ? c.nk : (c.nk - t + 1) >> 1; };
+  auto key_tile = [](const Piece& c, int t, int j) { return c.active == 2 ? j : 2 * j + t; };
+  // TMEM columns of a stream
   auto col_s = [](int t) { return (uint32_t)(t * TM); };
   auto col_o = [](int t) { return (uint32_t)(256 + t * D); };
   auto col_p = [](int t) { return (uint32_t)(D == 64 ? 384 + t * 64 : t * TM); };
@@ -210,198 +302,262 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     regs_dec<TC_LOW>();
     if (warp == 0) {
       // ------------------------------ producer ------------------------------
-      if (lane == 0) {
-        bar_expect_tx(q_full, active * SM::HALVES * p.group * tc.per_tile * 128);
-        for (int t = 0; t < active; ++t)
-          for (int h = 0; h < SM::HALVES; ++h)
-            tma_load_4d(&map_q, q_full, smem + SM::Q + t * SM::TILE + h * SM::HALF, h * 64, kh * p.group,
-                        tok0 + t * tc.per_tile, req);
-      }
       uint32_t* w = reinterpret_cast<uint32_t*>(smem + SM::ONES);
       for (int i = lane; i < XTILE * (1 + ST) / 4; i += 32) w[i] = 0u;
       __syncwarp();
       for (int row = lane; row < TM; row += 32)   // 1, 1, 1, 0, ...
         *reinterpret_cast<uint2*>(smem + SM::ONES + xtile_off(row, 0)) = make_uint2(0x3F803F80u, 0x3F80u);
-      const float* brow = p.bias ? p.bias + kh * p.bias_sh : nullptr;
+      fence_async_smem();
       const float inv_scale = 1.0f / p.scale, most = kBiasLimit / p.scale_log2;
-      float braw[4];
-      auto load_bias = [&](int j) {   // raw bias of a tile, one tile ahead of its use
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = (j0 + j) * TM + i * 32 + lane;
-          braw[i] = (brow && j0 + j < tp && key < p.prefix) ? __ldg(brow + key) : 0.f;
+      int i = 0, gk = 0, gv = 0;
+      bool okw = true;
+      Piece c;
+      for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+        done(turn);
+        if (c.nk == 0) continue;
+        if (i > 0 && !(okw = wait(q_empty, i - 1))) break;
+        if (lane == 0) {
+          bar_expect_tx(q_full, c.active * SM::HALVES * p.group * tc.per_tile * 128);
+          for (int t = 0; t < c.active; ++t)
+            for (int h = 0; h < SM::HALVES; ++h)
+              tma_load_4d(&map_q, q_full, smem + SM::Q + t * SM::TILE + h * SM::HALF, h * 64, c.kh * p.group,
+                          c.tok0 + t * tc.per_tile, c.req);
         }
-      };
-      load_bias(0);
-      int issued_k = 0, issued_v = 0;
-      for (int j = 0; j < nk; ++j) {
-        const int s = j % ST;
-        const uint32_t ph = (j / ST) & 1;
-        const Tile t = tile_of(j);
-        if (!wait(&k_empty[s], ph ^ 1)) break;
-        if (has_beta(t)) {
-          uint32_t* mask = reinterpret_cast<uint32_t*>(smem + SM::MASK + s * 16);
+        ++i;
+        const float* brow = p.bias ? p.bias + c.kh * p.bias_sh : nullptr;
+        float braw[4];
+        auto load_bias = [&](int j) {   // raw bias of a tile, one tile ahead of its use
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = i * 32 + lane;
-            const bool in = row < t.valid && braw[i] > -INFINITY;   // NaN takes a key out too
-            const float beta = in ? fminf(fmaxf(braw[i] * inv_scale, -most), most) : -INFINITY;
-            const __nv_bfloat16 hi = __float2bfloat16_rn(beta);
-            float rest = in ? beta - __bfloat162float(hi) : 0.f;
-            const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
-            rest -= __bfloat162float(mid);
-            *reinterpret_cast<uint2*>(smem + SM::BETA + s * XTILE + xtile_off(row, 0)) = make_uint2(
-                (uint32_t)__bfloat16_as_ushort(hi) | (uint32_t)__bfloat16_as_ushort(mid) << 16,
-                (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(rest)));
-            // rows to zero: own ones past the length, prefix ones by their bias
-            // (past the prefix's end the copy fills with zeros)
-            const unsigned out = __ballot_sync(0xffffffffu, !in && (t.own || row < t.valid));
-            if (lane == 0) mask[i] = out;
+          for (int u = 0; u < 4; ++u) {
+            const int key = (c.j0 + j) * TM + u * 32 + lane;
+            braw[u] = (brow && c.j0 + j < tp && key < p.prefix) ? __ldg(brow + key) : 0.f;
           }
-          fence_async_smem();
-          __syncwarp();
+        };
+        load_bias(0);
+        for (int j = 0; j < c.nk; ++j) {
+          const int s = gk % ST;
+          const uint32_t ph = gk / ST;
+          const Tile t = tile_of(c, j);
+          if (!(okw = wait(&k_empty[s], ph + 1))) break;
+          if (has_beta(t)) {
+            uint32_t* mask = reinterpret_cast<uint32_t*>(smem + SM::MASK + s * 16);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int row = u * 32 + lane;
+              const bool in = row < t.valid && braw[u] > -INFINITY;   // NaN takes a key out too
+              const float beta = in ? fminf(fmaxf(braw[u] * inv_scale, -most), most) : -INFINITY;
+              const __nv_bfloat16 hi = __float2bfloat16_rn(beta);
+              float rest = in ? beta - __bfloat162float(hi) : 0.f;
+              const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
+              rest -= __bfloat162float(mid);
+              *reinterpret_cast<uint2*>(smem + SM::BETA + s * XTILE + xtile_off(row, 0)) = make_uint2(
+                  (uint32_t)__bfloat16_as_ushort(hi) | (uint32_t)__bfloat16_as_ushort(mid) << 16,
+                  (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(rest)));
+              // rows to zero: own ones past the length, prefix ones by their bias
+              // (past the prefix's end the copy fills with zeros)
+              const unsigned out = __ballot_sync(0xffffffffu, !in && (t.own || row < t.valid));
+              if (lane == 0) mask[u] = out;
+            }
+            fence_async_smem();
+            __syncwarp();
+          }
+          load_bias(j + 1);
+          if (lane == 0) {
+            bar_expect_tx(&k_full[s], SM::TILE);
+            for (int h = 0; h < SM::HALVES; ++h)
+              tma_load_4d(t.own ? &map_ko : &map_kp, &k_full[s], smem + SM::K + s * SM::TILE + h * SM::HALF, h * 64,
+                          t.key0, c.kh, t.own ? c.req : 0);
+          }
+          ++gk;
+          if (!(okw = wait(&v_empty[s], ph + 1))) break;
+          if (lane == 0) {
+            bar_expect_tx(&v_full[s], SM::TILE);
+            for (int h = 0; h < SM::HALVES; ++h)
+              tma_load_4d(t.own ? &map_vo : &map_vp, &v_full[s], smem + SM::V + s * SM::TILE + h * SM::HALF, h * 64,
+                          t.key0, c.kh, t.own ? c.req : 0);
+          }
+          ++gv;
         }
-        load_bias(j + 1);
-        if (lane == 0) {
-          bar_expect_tx(&k_full[s], SM::TILE);
-          for (int h = 0; h < SM::HALVES; ++h)
-            tma_load_4d(t.own ? &map_ko : &map_kp, &k_full[s], smem + SM::K + s * SM::TILE + h * SM::HALF, h * 64,
-                        t.key0, kh, t.own ? req : 0);
-        }
-        issued_k = j + 1;
-        if (!wait(&v_empty[s], ph ^ 1)) break;
-        if (lane == 0) {
-          bar_expect_tx(&v_full[s], SM::TILE);
-          for (int h = 0; h < SM::HALVES; ++h)
-            tma_load_4d(t.own ? &map_vo : &map_vp, &v_full[s], smem + SM::V + s * SM::TILE + h * SM::HALF, h * 64,
-                        t.key0, kh, t.own ? req : 0);
-        }
-        issued_v = j + 1;
       }
       if (lane == 0) {   // copies in flight land before the CTA exits
         const unsigned long long t0 = global_ns();
-        drain_bar(q_full, 0, t0);
-        for (int j = max(0, issued_k - ST); j < issued_k; ++j) drain_bar(&k_full[j % ST], (j / ST) & 1, t0);
-        for (int j = max(0, issued_v - ST); j < issued_v; ++j) drain_bar(&v_full[j % ST], (j / ST) & 1, t0);
+        if (i > 0) drain_bar(q_full, (i - 1) & 1, t0);
+        for (int j = max(0, gk - ST); j < gk; ++j) drain_bar(&k_full[j % ST], (j / ST) & 1, t0);
+        for (int j = max(0, gv - ST); j < gv; ++j) drain_bar(&v_full[j % ST], (j / ST) & 1, t0);
       }
-    } else if (warp - 1 < streams) {
+    } else if (warp < 3) {
       // ------------------------------ MMA issuers ------------------------------
-      // j counts this stream's key tiles, key_tile(j) the chunk's
       const int t = warp - 1;
-      const int n = halves ? (nk - t + 1) >> 1 : nk;
-      auto key_tile = [&](int j) { return halves ? 2 * j + t : j; };
       const bool leader = elect_one();
       constexpr uint32_t idesc_s = idesc_bf16(TM, TM, false, false);
       constexpr uint32_t idesc_o = idesc_bf16(TM, D, false, true);
-      const uint64_t dQ = sdesc_sw128(smem_u32(smem + SM::Q + (halves ? 0 : t) * SM::TILE), 16, 1024);
+      const uint64_t dQ0 = sdesc_sw128(smem_u32(smem + SM::Q), 16, 1024);
       const uint64_t dK = sdesc_sw128(smem_u32(smem + SM::K), 16, 1024);
       const uint64_t dV = sdesc_sw128(smem_u32(smem + SM::V), SM::HALF, 1024);
       const uint64_t dOnes = sdesc_plain(smem_u32(smem + SM::ONES));
       const uint64_t dBeta = sdesc_plain(smem_u32(smem + SM::BETA));
       const uint32_t dS = tbase + col_s(t), dO = tbase + col_o(t), dP = tbase + col_p(t);
-      auto issue_s = [&](int j) {
-        const int jt = key_tile(j), st = jt % ST;
-        const bool beta = has_beta(tile_of(jt));
-        if (leader) {
-          const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
+      int i = 0, g = 0, cs = 0;   // cs: this stream's key tiles in earlier pieces
+      bool okw = true;
+      Piece c;
+      for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+        done(turn);
+        if (c.nk == 0) continue;
+        const int n = tiles_of(c, t);
+        const uint64_t dQ = dQ0 + (uint64_t)((c.active == 2 ? t : 0) * (SM::TILE >> 4));
+        auto issue_s = [&](int j) {
+          const int jt = key_tile(c, t, j), st = (g + jt) % ST;
+          const bool beta = has_beta(tile_of(c, jt));
+          if (leader) {
+            const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = (uint64_t)((k >> 2) * (SM::HALF >> 4) + (k & 3) * 2);
-            umma_bf16(dS, dQ + off, bk + off, idesc_s, k != 0);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t off = (uint64_t)((k >> 2) * (SM::HALF >> 4) + (k & 3) * 2);
+              umma_bf16(dS, dQ + off, bk + off, idesc_s, k != 0);
+            }
+            if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(st * (XTILE >> 4)), idesc_s, 1);
+            umma_commit(&s_full[t]);
+            umma_commit(&k_empty[st]);
+            if (c.active == 1) umma_commit(&k_empty[st]);
+            if (j == n - 1) umma_commit(q_empty);
           }
-          if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(st * (XTILE >> 4)), idesc_s, 1);
-          umma_commit(&s_full[t]);
-          umma_commit(&k_empty[st]);
-        }
-        __syncwarp();
-      };
-      auto issue_o = [&](int j) {
-        const int st = key_tile(j) % ST;
-        if (leader) {
-          const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
+          __syncwarp();
+        };
+        auto issue_o = [&](int j) {
+          const int st = (g + key_tile(c, t, j)) % ST;
+          if (leader) {
+            const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
-          for (int ks = 0; ks < TM / 16; ++ks)
-            umma_bf16_ts(dO, dP + ks * 8, bv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0));
-          umma_commit(&o_done[t]);
-          umma_commit(&v_empty[st]);
+            for (int ks = 0; ks < TM / 16; ++ks)
+              umma_bf16_ts(dO, dP + ks * 8, bv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0));
+            umma_commit(&o_done[t]);
+            umma_commit(&v_empty[st]);
+            if (c.active == 1) umma_commit(&v_empty[st]);
+          }
+          __syncwarp();
+        };
+        // The rows to zero of a key tile, read once its K has landed (the producer
+        // reuses the words before its V is used).
+        auto rows_out = [&](int j) {
+          const int jt = key_tile(c, t, j);
+          const Tile kt = tile_of(c, jt);
+          return (kt.own ? kt.valid < TM : p.bias != nullptr)
+                     ? *reinterpret_cast<const uint4*>(smem + SM::MASK + ((g + jt) % ST) * 16)
+                     : make_uint4(0u, 0u, 0u, 0u);
+        };
+        // Where both issuers read a tile, the second writes the same zeros.
+        auto zero_rows = [&](const uint4& m, int base, int j) {
+          if (!(m.x | m.y | m.z | m.w)) return;
+          uint8_t* tile =
+              smem + base + ((g + key_tile(c, t, j)) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
+          for (int row = 0; row < TM; ++row) {
+            const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
+            if ((word >> (row & 31) & 1) && lane < 8 * SM::HALVES)
+              *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+        };
+        auto wait_tile = [&](uint64_t* bar, int j) {
+          const int gt = g + key_tile(c, t, j);
+          return wait(&bar[gt % ST], gt / ST);
+        };
+        uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
+        auto scores = [&](int j) {   // once K has landed and S is free
+          tc_fence_after();
+          out_next = rows_out(j);
+          zero_rows(out_next, SM::K, j);
+          issue_s(j);
+        };
+        okw = wait(q_full, i);
+        if (okw && n == 0 && leader) bar_arrive(q_empty);   // nothing to read for this stream
+        if (okw && n > 0) {
+          // S is free once the last softmax has read it, or (P in its place) the last product with V is done
+          okw = wait_tile(k_full, 0) && (cs == 0 || wait(D == 64 ? &s_empty[t] : &o_done[t], cs - 1));
+          if (okw) scores(0);
         }
-        __syncwarp();
-      };
-      // The rows to zero of a key tile, read once its K has landed (the producer
-      // reuses the words before its V is used).
-      auto rows_out = [&](int j) {
-        const Tile kt = tile_of(key_tile(j));
-        return (kt.own ? kt.valid < TM : p.bias != nullptr)
-                   ? *reinterpret_cast<const uint4*>(smem + SM::MASK + (key_tile(j) % ST) * 16)
-                   : make_uint4(0u, 0u, 0u, 0u);
-      };
-      // Where both issuers read a tile, the second writes the same zeros.
-      auto zero_rows = [&](const uint4& m, int base, int j) {
-        if (!(m.x | m.y | m.z | m.w)) return;
-        uint8_t* tile = smem + base + (key_tile(j) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
-        for (int row = 0; row < TM; ++row) {
-          const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
-          if ((word >> (row & 31) & 1) && lane < 8 * SM::HALVES)
-            *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_async_smem();
-        __syncwarp();
-      };
-      auto wait_tile = [&](uint64_t* bar, int j) { return wait(&bar[key_tile(j) % ST], key_tile(j) / ST); };
-      uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
-      auto scores = [&](int j) {   // once K has landed
-        tc_fence_after();
-        out_next = rows_out(j);
-        zero_rows(out_next, SM::K, j);
-        issue_s(j);
-      };
-      bool okw = wait(q_full, 0) && wait_tile(k_full, 0);
-      if (okw) scores(0);
-      for (int j = 0; okw && j < n; ++j) {
-        out_now = out_next;
-        if (D == 64 && j + 1 < n) {
-          okw = wait(&s_empty[t], j) && wait_tile(k_full, j + 1);
+        for (int j = 0; okw && j < n; ++j) {
+          out_now = out_next;
+          if (D == 64 && j + 1 < n) {
+            okw = wait(&s_empty[t], cs + j) && wait_tile(k_full, j + 1);
+            if (!okw) break;
+            scores(j + 1);
+          }
+          okw = wait(&p_full[t], cs + j) && wait_tile(v_full, j);
           if (!okw) break;
-          scores(j + 1);
+          tc_fence_after();
+          zero_rows(out_now, SM::V, j);
+          issue_o(j);
+          if (D == 128 && j + 1 < n) {
+            // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
+            okw = wait_tile(k_full, j + 1) && wait(&o_done[t], cs + j);
+            if (!okw) break;
+            scores(j + 1);
+          }
         }
-        okw = wait(&p_full[t], j) && wait_tile(v_full, j);
-        if (!okw) break;
-        tc_fence_after();
-        zero_rows(out_now, SM::V, j);
-        issue_o(j);
-        if (D == 128 && j + 1 < n) {
-          // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
-          okw = wait_tile(k_full, j + 1) && wait(&o_done[t], j);
-          if (!okw) break;
-          scores(j + 1);
+        ++i;
+        g += c.nk;
+        cs += n;
+      }
+    } else {
+      // ------------------------------ planner ------------------------------
+      walk.req = start_req;
+      walk.req0 = start_req0;
+      Piece c;
+      for (uint32_t turn = 0;; ++turn) {
+        const bool more = next_piece(p, tc, walk, c);
+        if (!wait(&piece_empty[turn % RING], turn / RING + 1)) break;
+        if (lane == 0) {
+          if (!more) c.req = -1;
+          ring[turn % RING] = c;
+          bar_arrive(&piece_full[turn % RING]);
         }
+        if (!more) break;
       }
     }
   } else {
     regs_inc<TC_HIGH>();
     // ------------------------------ softmax ------------------------------
     const int t = (warp - 4) >> 2;
-    if (t < streams) {
-      const int n = halves ? (nk - t + 1) >> 1 : nk;
-      const int quad = warp & 3;
-      const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-      const uint32_t tS = tbase + lane_off + col_s(t), tO = tbase + lane_off + col_o(t), tP = tbase + lane_off + col_p(t);
-      const Row row = row_of(halves ? 0 : t, quad * 32 + lane);
+    const int quad = warp & 3;
+    const int row_i = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t tS = tbase + lane_off + col_s(t), tO = tbase + lane_off + col_o(t), tP = tbase + lane_off + col_p(t);
+    float2* half_ml = reinterpret_cast<float2*>(smem + SM::ML) + row_i;
+    const float c2 = p.scale_log2;
+    constexpr float kNoMax = -3.0e38f;   // no key yet
+    const int tl = row_i / p.group, head = row_i - tl * p.group;
+    int cs = 0, ih = 0;   // ih: pieces in halves so far
+    bool okw = true;
+    Piece c;
+    for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+      const int n = tiles_of(c, t);
+      const bool halves = c.active == 1 && c.nk > 1;
+      // this thread's row
+      Row row;
+      {
+        const int tok = c.tok0 + (c.active == 2 ? t : 0) * tc.per_tile + tl;
+        row.h = c.kh * p.group + head;
+        row.live = tl < tc.per_tile && tok < c.tok_end;
+        row.r = c.req;
+        row.m = tok;
+        if (tc.fold) {
+          row.r = tok / p.queries;
+          row.m = tok - row.r * p.queries;
+          if (row.live && p.q_len) row.live = row.m < __ldg(p.q_len + row.r);
+        }
+      }
       const bool idle = !__any_sync(0xffffffffu, row.live);   // a warp without rows only keeps the barriers going
       // own keys that this row sees end here
-      const bool ordered = p.causal && !tc.fold;
-      const int limit = ordered ? len - qlen + row.m + 1 : 0x7fffffff;
-      constexpr float kNoMax = -3.0e38f;   // no key yet
+      const int limit = CAUSAL ? c.len - c.qlen + row.m + 1 : 0;
       float m_raw = kNoMax, l = 0.f;       // running maximum (score units), row sum
       float neg_mc = 0.f;                  // -c2 * m_raw
-      const float c2 = p.scale_log2;
-      bool okw = true;
-      auto quarter = [&](float* xq, float neg_mc, float* acc, uint32_t* pk) {
+      auto quarter = [&](float* xq, float neg, float* acc, uint32_t* pk) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float* xg = xq + g * 8;
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) ffma2(xg[i], xg[i + 1], xg[i], xg[i + 1], c2, c2, neg_mc, neg_mc);
+          for (int i = 0; i < 8; i += 2) ffma2(xg[i], xg[i + 1], xg[i], xg[i + 1], c2, c2, neg, neg);
           float e[8];
           exp8(xg, e);
 #pragma unroll
@@ -412,8 +568,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       };
       if (idle) {
         for (int j = 0; j < n; ++j) {
-          // S(j+1) may be there before the other warps' P(j): no second arrival in one phase
-          okw = wait(&s_full[t], j) && (j == 0 || wait(&p_full[t], j - 1));
+          // the next S may be there before the other warps' P: no second arrival in one phase
+          okw = wait(&s_full[t], cs + j) && (cs + j == 0 || wait(&p_full[t], cs + j - 1));
           if (!okw) break;
           if (lane == 0) {
             if (D == 64) bar_arrive(&s_empty[t]);
@@ -422,29 +578,29 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
       }
       for (int j = idle ? n : 0; j < n; ++j) {
-        if (!wait(&s_full[t], j)) { okw = false; break; }
+        if (!wait(&s_full[t], cs + j)) { okw = false; break; }
         tc_fence_after();
         float x[TM];
 #pragma unroll
-        for (int c = 0; c < TM / 32; ++c) tmem_ld32f(tS + c * 32, x + c * 32);
+        for (int u = 0; u < TM / 32; ++u) tmem_ld32f(tS + u * 32, x + u * 32);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
-        if (ordered) {   // keys ahead of this row
-          const Tile kt = tile_of(halves ? 2 * j + t : j);
+        if (CAUSAL) {   // keys ahead of this row
+          const Tile kt = tile_of(c, key_tile(c, t, j));
           if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {
             const int end = limit - kt.key0;
 #pragma unroll
-            for (int c = 0; c < TM; ++c)
-              if (c >= end) x[c] = -INFINITY;
+            for (int u = 0; u < TM; ++u)
+              if (u >= end) x[u] = -INFINITY;
           }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < TM / 4; ++c) {
-          mx[c & 3] = max3_nan(mx[c & 3], x[4 * c + 0], x[4 * c + 1]);
-          mx[c & 3] = max3_nan(mx[c & 3], x[4 * c + 2], x[4 * c + 3]);
+        for (int u = 0; u < TM / 4; ++u) {
+          mx[u & 3] = max3_nan(mx[u & 3], x[4 * u + 0], x[4 * u + 1]);
+          mx[u & 3] = max3_nan(mx[u & 3], x[4 * u + 2], x[4 * u + 3]);
         }
         const float mt = max3_nan(max3_nan(mx[0], mx[0], mx[1]), mx[2], mx[3]);
         float alpha = 1.f;
@@ -468,7 +624,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             tmem_st16(tP + qt * 16, pk[qt]);
           } else if (qt == 1) {
             if (j > 0) {    // P and O are busy until O += P(j-1) V is done
-              if (!wait(&o_done[t], j - 1)) { okw = false; break; }
+              if (!wait(&o_done[t], cs + j - 1)) { okw = false; break; }
               tc_fence_after();
             }
             tmem_st16(tP, pk[0]);
@@ -482,12 +638,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (j > 0 && any_moved) {
           uint32_t ov[32];
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            tmem_ld32(tO + c * 32, ov);
+          for (int u = 0; u < D / 32; ++u) {
+            tmem_ld32(tO + u * 32, ov);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-            tmem_st32(tO + c * 32, ov);
+            tmem_st32(tO + u * 32, ov);
           }
         }
         tmem_wait_st();
@@ -495,75 +651,95 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(&p_full[t]);
       }
-      if (okw) okw = wait(&o_done[t], n - 1);
+      cs += n;
+      if (okw && n > 0) okw = wait(&o_done[t], cs - 1);
       tc_fence_after();
-      // The second half's output goes through the rings' memory (all of it has
-      // been read once both halves are done), feature-major: a thread per row.
-      float* xo = reinterpret_cast<float*>(smem + SM::K) + quad * 32 + lane;
-      float* xml = reinterpret_cast<float*>(smem + SM::Q) + (quad * 32 + lane) * 2;
-      float f1 = 0.f;
-      if (halves) {
-        named_sync();
-        if (t == 1 && okw) {
-          xml[0] = m_raw;
-          xml[1] = l;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t ov[32];
-            tmem_ld32(tO + c * 32, ov);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) xo[(c * 32 + i) * TM] = __uint_as_float(ov[i]);
-          }
+      if (halves && t == 1) {   // hand over this half: O stays in TMEM until it is read
+        if (okw) {
+          *half_ml = make_float2(m_raw, l);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(half_there);
+          okw = wait(half_read, ih);
         }
-        named_sync();
+        ++ih;
+        done(turn);
+        continue;
       }
-      if (okw && !*abort_flag && !(halves && t == 1)) {
-        float f0 = 1.f;
-        if (halves) {
-          const float m1 = xml[0], m = fmaxf(m_raw, m1);
+      if (c.active == 1 && t == 1) {
+        done(turn);
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if (halves) {
+        okw = okw && wait(half_there, ih);
+        ++ih;
+        if (okw) {
+          tc_fence_after();
+          const float2 other = *half_ml;
+          const float m = fmaxf(m_raw, other.x);
           f0 = fast_exp2((m_raw - m) * c2);
-          f1 = fast_exp2((m1 - m) * c2);
-          l = l * f0 + xml[1] * f1;
+          f1 = fast_exp2((other.x - m) * c2);
+          l = l * f0 + other.y * f1;
           m_raw = m;
         }
-        const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
-        const float inv = some ? 1.0f / l : 0.f;
-        const int64_t at = split * p.rows + row_index(p, row);
-        __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
+      }
+      if (!okw || *abort_flag) break;
+      const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
+      const float inv = some ? 1.0f / l : 0.f;
+      const bool direct = c.first && c.last && p.s2 == 0;
+      const int64_t at = row_index(p, row), to = c.slot * p.rows + at;
+      __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
+      if (!idle) {
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t ov[32];
-          tmem_ld32(tO + c * 32, ov);
-          tmem_wait_ld();
-          if (!row.live) continue;
+        for (int u = 0; u < D / 32; ++u) {
           float v[32];
+          {
+            uint32_t ov[32];
+            if (n > 0) {
+              tmem_ld32(tO + u * 32, ov);
+              tmem_wait_ld();
+            }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ov[i]);
-          if (halves) {
+            for (int i = 0; i < 32; ++i) v[i] = n > 0 ? __uint_as_float(ov[i]) : 0.f;
+            if (halves) {
+              tmem_ld32(tbase + lane_off + col_o(1) + u * 32, ov);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], f0, xo[(c * 32 + i) * TM] * f1);
+              for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], f0, __uint_as_float(ov[i]) * f1);
+            }
           }
-          if (partial) {
-            float4* w = reinterpret_cast<float4*>(p.ws_o + at * D + c * 32);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) w[u] = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-          } else {
+          if (!row.live) continue;
+          if (direct) {
             uint32_t w[16];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) w[u] = some ? pack_bf16x2(v[2 * u] * inv, v[2 * u + 1] * inv) : 0u;
+            for (int i = 0; i < 16; ++i) w[i] = some ? pack_bf16x2(v[2 * i] * inv, v[2 * i + 1] * inv) : 0u;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              reinterpret_cast<uint4*>(orow + c * 32)[u] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(orow + u * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else if (some) {
+            float4* w = reinterpret_cast<float4*>(p.ws_o + to * D + u * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         }
-        if (row.live) {
-          if (partial)
-            p.ws_ml[at] = some ? make_float2(m_raw * c2, l) : make_float2(-INFINITY, 0.f);
-          else if (p.lse)
-            p.lse[row.r * p.lse_sr + row.h * p.lse_sh + row.m] = some ? m_raw * c2 + log2f(l) : -INFINITY;
+      }
+      if (halves) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(half_read);
+      }
+      if (row.live) {
+        if (direct) {
+          if (p.lse) p.lse[row.r * p.lse_sr + row.h * p.lse_sh + row.m] = some ? m_raw * c2 + log2f(l) : -INFINITY;
+          p.ws_ml[at] = make_float2(0.f, kWritten);
+        } else {
+          p.ws_ml[to] = some ? make_float2(m_raw * c2, l) : make_float2(-INFINITY, 0.f);
+          if (c.last)   // slots that no piece of this item takes
+            for (int s = c.slot + 1; s < p.s1; ++s) p.ws_ml[s * p.rows + at] = make_float2(-INFINITY, 0.f);
         }
       }
+      done(turn);
     }
   }
   tc_fence_before();
@@ -604,21 +780,21 @@ bool tc_takes(const Params& p, int head_dim, bool fold) {
 
 // The register split needs a launch with TC_REGS registers per thread; refuse
 // to launch otherwise (it would never start).
-template <int D>
+template <int D, bool CAUSAL>
 static int check_regs() {
   cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, tc_kernel<D>) != cudaSuccess)
+  if (cudaFuncGetAttributes(&fa, tc_kernel<D, CAUSAL>) != cudaSuccess)
     return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: cudaFuncGetAttributes failed");
   if (fa.numRegs * TC_THREADS < TC_LOW * 128 + TC_HIGH * 256)
     return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: kernel built with %d registers/thread", fa.numRegs);
   return GPA_OK;
 }
 
-template <int D>
+template <int D, bool CAUSAL>
 static int launch(const Params& p, const TcPlan& t, cudaStream_t st) {
   static bool checked = false;
   if (!checked) {
-    const int rc = check_regs<D>();
+    const int rc = check_regs<D, CAUSAL>();
     if (rc) return rc;
     checked = true;
   }
@@ -635,15 +811,15 @@ static int launch(const Params& p, const TcPlan& t, cudaStream_t st) {
   if (rc) return rc;
   if (!pre) mkp = mko, mvp = mvo;   // never read
   if (!own) mko = mkp, mvo = mvp;
-  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D>::ALLOC);
+  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D>::ALLOC);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
-  const int64_t items = (int64_t)t.pairs * nreq * t.splits * p.kv_heads;
-  tc_kernel<D><<<(unsigned)items, TC_THREADS, TcSmem<D>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
+  tc_kernel<D, CAUSAL><<<t.ctas, TC_THREADS, TcSmem<D>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
   return check_launch("gpa_attention_shared_prefix");
 }
 
 int launch_tc(const Params& p, int head_dim, const TcPlan& t, cudaStream_t st) {
-  return head_dim == 64 ? launch<64>(p, t, st) : launch<128>(p, t, st);
+  if (p.causal && !t.fold) return head_dim == 64 ? launch<64, true>(p, t, st) : launch<128, true>(p, t, st);
+  return head_dim == 64 ? launch<64, false>(p, t, st) : launch<128, false>(p, t, st);
 }
 
 }  // namespace prefix

@@ -25,7 +25,7 @@ constexpr int BN = 64;         // keys per tile
 constexpr int THREADS = 128;
 constexpr int kSlotTiles = 4;  // at least this many tiles per chunk
 constexpr int kSms = 148;
-constexpr int kLeastSpan = 4;  // at least this many steps per CTA of the tensor-core kernel
+constexpr int kLeastSteps = 4;  // at least this many steps per CTA of the tensor-core kernel
 
 template <int D>
 struct Cfg {
@@ -358,23 +358,16 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   run_item<D, WM2, true>(p, smem, (int)(it % p.kv_heads), (int)(it / p.kv_heads), t, s);
 }
 
-// Joins a row's chunks.  W warps per row: one for a few chunks, eight (a block)
-// for many, each taking every eighth chunk.  The launch overlaps the end of the
-// kernel before it (a programmatic dependency), which the first line waits for.
+// Joins the chunks of a row with W warps (1: a warp's own row, 8: the block's).
 template <int D, int W>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+__device__ __forceinline__ void join_row(const Params& p, int64_t row, float (*part)[D]) {
   constexpr int F = D / 32;   // features per lane
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
-  if (row >= p.rows) return;
   const int h = (int)((uint32_t)row % (uint32_t)p.heads), tok = (int)((uint32_t)row / (uint32_t)p.heads);
   const int m = (int)((uint32_t)tok % (uint32_t)p.queries), r = (int)((uint32_t)tok / (uint32_t)p.queries);
-  if (p.q_len && m >= __ldg(p.q_len + r)) return;
   const int slots = p.s1 + p.s2;
   const float2* mlr = p.ws_ml + row;
   const float2 first = lane < slots ? mlr[lane * p.rows] : make_float2(-INFINITY, 0.f);
-  if (__shfl_sync(0xffffffffu, first.y, 0) == kWritten) return;   // by the tensor-core kernel
   float mx = first.x;
   for (int s = lane + 32; s < slots; s += 32) mx = fmaxf(mx, mlr[s * p.rows].x);
 #pragma unroll
@@ -419,7 +412,6 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   if constexpr (W > 1) {
-    __shared__ float part[W][D];
 #pragma unroll
     for (int u = 0; u < F; ++u) part[warp][lane * F + u] = v[u];
     __syncthreads();
@@ -441,20 +433,52 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   if (p.lse && lane == 0) p.lse[r * p.lse_sr + h * p.lse_sh + m] = l == 0.f ? -INFINITY : mx + log2f(l);
 }
 
+// Whether a row's chunks are to be joined: not past its request's queries, nor
+// written by the tensor-core kernel already.
+__device__ __forceinline__ bool to_join(const Params& p, int64_t row) {
+  if (row >= p.rows) return false;
+  if (p.q_len) {
+    const uint32_t tok = (uint32_t)row / (uint32_t)p.heads;
+    if ((int)(tok % (uint32_t)p.queries) >= __ldg(p.q_len + tok / (uint32_t)p.queries)) return false;
+  }
+  return p.s1 + p.s2 == 0 || p.ws_ml[row].y != kWritten;
+}
+
+// WIDE: a block per row, each warp taking every eighth chunk.  Else RPW rows per
+// warp: most rows of a large call are written already, and a look at RPW of them
+// at once finds the others.  The launch overlaps the end of the kernel before it
+// (a programmatic dependency), which the first line waits for.
+template <int D, bool WIDE, int RPW>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (WIDE) {
+    __shared__ float part[8][D];
+    if (to_join(p, blockIdx.x)) join_row<D, 8>(p, blockIdx.x, part);
+  } else {
+    const int lane = threadIdx.x & 31;
+    const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW;
+    unsigned left = __ballot_sync(0xffffffffu, lane < RPW && to_join(p, row0 + lane));
+    for (; left; left &= left - 1) join_row<D, 1>(p, row0 + __ffs(left) - 1, nullptr);
+  }
+}
+
 template <int D>
 static int launch_join(const Params& p, cudaStream_t st) {
-  // eight warps per row from where one would go twice through its eight loads
-  const bool wide = p.s1 + p.s2 > 16;
+  // eight warps per row from where one would go twice through its eight loads,
+  // several rows per warp from where they fill the GPU all the same
+  const bool wide = p.s1 + p.s2 > 16 && p.rows <= 16384, many = !wide && p.rows > 32768;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(wide ? p.rows : (p.rows + 7) / 8));
+  cfg.gridDim = dim3((unsigned)(wide ? p.rows : many ? (p.rows + 127) / 128 : (p.rows + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, join_kernel<D, 8>, p) : cudaLaunchKernelEx(&cfg, join_kernel<D, 1>, p);
+  const cudaError_t e = wide   ? cudaLaunchKernelEx(&cfg, join_kernel<D, true, 1>, p)
+                        : many ? cudaLaunchKernelEx(&cfg, join_kernel<D, false, 16>, p)
+                               : cudaLaunchKernelEx(&cfg, join_kernel<D, false, 1>, p);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
   return check_launch("gpa_attention_shared_prefix");
 }
@@ -486,18 +510,22 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
     p.tc.fold = fold;
     p.tc.tokens = fold ? requests * queries : queries;
     p.tc.per_tile = 128 / group;
-    // The steps of all items at full lengths (the kernel counts the real ones),
-    // and what a CTA gets of them.  An item is cut where a span ends: at most
-    // steps / span + 2 parts; twice the steps / span leaves room for spans that
+    // The units of all items at full lengths (the kernel counts the real ones),
+    // and what a CTA gets of them.  An item is cut where a span ends: into at most
+    // units / span + 2 parts; twice the units / span leaves room for spans that
     // shorter lengths make shorter.
     const int64_t tiles = (p.tc.tokens + p.tc.per_tile - 1) / p.tc.per_tile;
-    const int64_t steps = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
-    const int64_t total = ((tiles >> 1) * steps + (tiles & 1 ? (steps + 1) / 2 : 0)) * kv_heads * (fold ? 1 : requests);
-    const int64_t span = std::max<int64_t>((total + kSms - 1) / kSms, kLeastSpan);
-    const int64_t cuts = std::min<int64_t>(2 * ((steps + span - 1) / span), std::max<int64_t>(steps / kLeastSpan, 1));
-    p.tc.least = (int)std::max<int64_t>((steps + cuts - 1) / cuts, kLeastSpan);
-    p.tc.ctas = (int)std::min<int64_t>(kSms, (total + kLeastSpan - 1) / kLeastSpan);
-    p.s1 = (int)((steps + p.tc.least - 1) / p.tc.least) + 1;
+    const int64_t keys = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
+    p.tc.halves = tiles == 1;
+    const int64_t steps = p.tc.halves ? (keys + 1) / 2 : keys;
+    const int each = tiles > 1 ? kPair : kSingle;
+    const int64_t units = steps * each, least = kLeastSteps * each;
+    const int64_t total = (tiles / 2 * kPair + tiles % 2 * kSingle) * steps * kv_heads * (fold ? 1 : requests);
+    const int64_t span = std::max((total + kSms - 1) / kSms, least);
+    const int64_t cuts = std::min(2 * ((units + span - 1) / span), std::max<int64_t>(units / least, 1));
+    p.tc.least = (int)std::min<int64_t>(std::max((units + cuts - 1) / cuts, least), 1 << 30);
+    p.tc.ctas = (int)std::min<int64_t>(kSms, (total + least - 1) / least);
+    p.s1 = (int)((units + p.tc.least - 1) / p.tc.least) + 1;
   }
   if (p.rows_run) {
     const int64_t t1 = p.tc_run ? 0 : (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;

@@ -48,13 +48,17 @@ __device__ __forceinline__ int query_count(const Params& p, int r) {
 // What the sum of a row's first partial output holds when its output is written.
 constexpr float kWritten = -1.0f;
 
+// Units of time that a step of it counts, with rows in two tiles or in one.
+constexpr int kPair = 3, kSingle = 2;
+
 // The tensor-core kernel's share of a call: 2 x 128-row tiles over the prefix
 // and, unless `fold`, each request's own keys.
 struct TcPlan {
   int fold;      // rows run through all requests (prefix only), else within one request
   int tokens;    // tokens a tile's rows may come from: requests * queries (fold) or queries
   int per_tile;  // tokens of a 128-row tile
-  int ctas;      // each takes a span of the key-tile steps
+  int halves;    // every item has rows in one tile only
+  int ctas;      // each takes a span of the units of work
   int least;     // of at least so many: no item is cut into more than s1 parts
 };
 // Whether the kernel can take the call's strides and scale.

@@ -5,9 +5,10 @@
 // tiles: the prefix's, then the request's own ones, in one online softmax.  One
 // CTA per SM; the items' key tiles, laid end to end, are dealt out in equal spans,
 // so that a CTA may begin and end inside an item (its part is joined later) and
-// no wave is left half empty: the lengths on the device set the spans.  A pair of
-// which only one tile has rows runs it over the even and the odd key tiles at
-// once instead.  384 threads:
+// no wave is left half empty: the lengths on the device set the spans.  Calls of
+// which every item has rows in one tile only (HALVES) run it over the even and the
+// odd key tiles at once instead; elsewhere the softmax of the tile that an item may
+// lack at its end is left out.  384 threads:
 //   warp 0     TMA producer: Q, then K and V tiles of 128 keys through a ring
 //              each, on into the next item; writes a tile's bias / scale as three
 //              bf16 terms (24 bits) that one more K=16 step adds to the scores,
@@ -88,73 +89,82 @@ __device__ __forceinline__ void exp8(const float* x, float* e) {
 }
 
 // The order of work: requests, their key heads, the head's row-tile pairs, a
-// pair's steps.  A step is one key tile for two row tiles or two for one.
+// pair's steps (a key tile; two of them in halves).  A step of a pair with two
+// row tiles counts three units of time, of one two.
 struct Load {
   int pairs2;      // pairs with two row tiles
   bool single;     // and one with one
-  int nk;          // key tiles (none at all counts as one, to write the empty rows)
-  int64_t head;    // steps of one key head
+  int steps;       // of a pair (no keys at all count as one, to write the empty rows)
+  int64_t head;    // units of one key head
 };
+template <bool HALVES>
 __device__ __forceinline__ Load load_of(const Params& p, const TcPlan& tc, int r) {
   Load w;
   const int tokens = tc.fold ? tc.tokens : query_count(p, r);
   const int tiles = (tokens + tc.per_tile - 1) / tc.per_tile;
   w.pairs2 = tiles >> 1;
   w.single = tiles & 1;
-  w.nk = max(1, (p.prefix + TM - 1) / TM + (tc.fold ? 0 : (own_length(p, r) + TM - 1) / TM));
-  w.head = (int64_t)w.pairs2 * w.nk + (w.single ? (w.nk + 1) >> 1 : 0);
+  const int keys = max(1, (p.prefix + TM - 1) / TM + (tc.fold ? 0 : (own_length(p, r) + TM - 1) / TM));
+  w.steps = HALVES ? (keys + 1) >> 1 : keys;
+  w.head = (int64_t)w.steps * (kPair * w.pairs2 + (w.single ? kSingle : 0));
   return w;
 }
 
 // A CTA's share of one item.
 struct Piece {
   int req, kh, tok0, tok_end;
-  int active;        // row tiles with rows: 1 or 2
   int len, qlen;
   int j0, nk;        // key tiles (nk may be 0: nothing to see here)
   int slot;          // which partial output
   bool first, last;  // holds the item's first, last step
 };
 struct Walk {
-  int64_t pos, end, span;   // this CTA's steps
+  int64_t pos, end, span;   // this CTA's units
   int req;
-  int64_t req0;             // first step of the request
+  int64_t req0;             // first unit of the request
 };
+template <bool HALVES>
 __device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Walk& w, Piece& c) {
-  if (w.pos >= w.end) return false;
-  Load ld = load_of(p, tc, w.req);
-  while (w.pos - w.req0 >= ld.head * p.kv_heads) {
-    w.req0 += ld.head * p.kv_heads;
-    ld = load_of(p, tc, ++w.req);
-  }
-  const int64_t x = w.pos - w.req0;
+  int a, b, steps;
+  do {
+    if (w.pos >= w.end) return false;
+    Load ld = load_of<HALVES>(p, tc, w.req);
+    while (w.pos - w.req0 >= ld.head * p.kv_heads) {
+      w.req0 += ld.head * p.kv_heads;
+      ld = load_of<HALVES>(p, tc, ++w.req);
+    }
+    const int64_t x = w.pos - w.req0;
+    c.kh = (int)(x / ld.head);
+    const int64_t y = x - c.kh * ld.head;
+    steps = ld.steps;
+    const int pair = (int)min(y / (kPair * (int64_t)steps), (int64_t)ld.pairs2);
+    const int64_t at = y - pair * (kPair * (int64_t)steps);   // units of the pair that others have
+    const int each = pair < ld.pairs2 ? kPair : kSingle;
+    const int64_t units = min((int64_t)steps * each - at, w.end - w.pos);
+    // a step goes to the CTA that has its first unit
+    a = (int)((at + each - 1) / each);
+    b = (int)((at + units + each - 1) / each);
+    c.slot = (int)(blockIdx.x - (w.pos - at) / w.span);
+    c.tok0 = pair * 2 * tc.per_tile;
+    w.pos += units;
+  } while (a == b);   // the rest of a step that the CTA before has done
   c.req = w.req;
-  c.kh = (int)(x / ld.head);
-  const int64_t y = x - c.kh * ld.head;
-  const int pair = (int)min(y / ld.nk, (int64_t)ld.pairs2);
-  const int a = (int)(y - (int64_t)pair * ld.nk);
-  c.active = pair < ld.pairs2 ? 2 : 1;
-  const int steps = c.active == 2 ? ld.nk : (ld.nk + 1) >> 1;
-  const int b = (int)min((int64_t)steps, a + (w.end - w.pos));
-  c.tok0 = pair * 2 * tc.per_tile;
   c.qlen = tc.fold ? p.queries : query_count(p, c.req);
   c.tok_end = tc.fold ? tc.tokens : c.qlen;
   c.len = tc.fold ? 0 : own_length(p, c.req);
   // with an order, no row of this pair sees an own key from here on
   const int own_end =
       p.causal ? min(c.len, max(0, c.len - c.qlen + min(c.tok0 + 2 * tc.per_tile, c.qlen))) : c.len;
-  const int tiles = (p.prefix + TM - 1) / TM + (own_end + TM - 1) / TM, each = 3 - c.active;
+  const int tiles = (p.prefix + TM - 1) / TM + (own_end + TM - 1) / TM, each = HALVES ? 2 : 1;
   c.j0 = a * each;
   c.nk = max(0, min(tiles, b * each) - c.j0);
   c.first = a == 0;
   c.last = b == steps;
-  c.slot = (int)(blockIdx.x - (w.pos - a) / w.span);
-  w.pos += b - a;
   return true;
 }
 
 // CAUSAL: own keys in order (a kernel of its own: the mask costs the others registers).
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, bool HALVES>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kp,
               const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_ko,
@@ -162,14 +172,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   using SM = TcSmem<D>;
   constexpr int ST = SM::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ int64_t warp_steps[TC_THREADS / 32];
+  __shared__ int64_t warp_units[TC_THREADS / 32];
   __shared__ int64_t start_req0;
   __shared__ int start_req;
   __shared__ Piece ring[RING];
   asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
   const int warp = warp_id(), lane = lane_id();
 
-  // All steps, this CTA's span of them, and the request that it starts in: each
+  // All units, this CTA's span of them, and the request that it starts in: each
   // thread adds up a run of requests.
   Walk walk;
   {
@@ -177,19 +187,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int run = (nreq + TC_THREADS - 1) / TC_THREADS;
     const int r0 = threadIdx.x * run, r1 = min(nreq, r0 + run);
     int64_t mine = 0;
-    for (int r = r0; r < r1; ++r) mine += load_of(p, tc, r).head * p.kv_heads;
+    for (int r = r0; r < r1; ++r) mine += load_of<HALVES>(p, tc, r).head * p.kv_heads;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    if (lane == 31) warp_steps[warp] = upto;
+    if (lane == 31) warp_units[warp] = upto;
     __syncthreads();
     int64_t before = 0, total = 0;
     for (int i = 0; i < TC_THREADS / 32; ++i) {
-      if (i < warp) before += warp_steps[i];
-      total += warp_steps[i];
+      if (i < warp) before += warp_units[i];
+      total += warp_units[i];
     }
     walk.span = max((total + gridDim.x - 1) / gridDim.x, (int64_t)tc.least);
     walk.pos = blockIdx.x * walk.span;
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (walk.pos >= at && walk.pos < at + mine) {
       int r = r0;
       for (;; ++r) {
-        const int64_t n = load_of(p, tc, r).head * p.kv_heads;
+        const int64_t n = load_of<HALVES>(p, tc, r).head * p.kv_heads;
         if (walk.pos < at + n) break;
         at += n;
       }
@@ -235,8 +245,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       bar_init(&k_full[s], 1);
       bar_init(&v_full[s], 1);
-      bar_init(&k_empty[s], 2);   // one arrival per row tile, or two by the one stream that reads the tile
-      bar_init(&v_empty[s], 2);
+      bar_init(&k_empty[s], HALVES ? 1 : 2);   // one arrival per row tile
+      bar_init(&v_empty[s], HALVES ? 1 : 2);
     }
     for (int t = 0; t < 2; ++t) {
       bar_init(&s_full[t], 1);
@@ -291,8 +301,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   };
   auto has_beta = [&](const Tile& t) { return t.valid < TM || (!t.own && p.bias != nullptr); };
   // key tiles of stream t, and which they are
-  auto tiles_of = [](const Piece& c, int t) { return c.active == 2 ? c.nk : (c.nk - t + 1) >> 1; };
-  auto key_tile = [](const Piece& c, int t, int j) { return c.active == 2 ? j : 2 * j + t; };
+  auto tiles_of = [](const Piece& c, int t) { return HALVES ? (c.nk - t + 1) >> 1 : c.nk; };
+  auto key_tile = [](int t, int j) { return HALVES ? 2 * j + t : j; };
   // TMEM columns of a stream
   auto col_s = [](int t) { return (uint32_t)(t * TM); };
   auto col_o = [](int t) { return (uint32_t)(256 + t * D); };
@@ -317,8 +327,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (c.nk == 0) continue;
         if (i > 0 && !(okw = wait(q_empty, i - 1))) break;
         if (lane == 0) {
-          bar_expect_tx(q_full, c.active * SM::HALVES * p.group * tc.per_tile * 128);
-          for (int t = 0; t < c.active; ++t)
+          constexpr int TILES = HALVES ? 1 : 2;   // past the last token the copy fills with zeros
+          bar_expect_tx(q_full, TILES * SM::HALVES * p.group * tc.per_tile * 128);
+          for (int t = 0; t < TILES; ++t)
             for (int h = 0; h < SM::HALVES; ++h)
               tma_load_4d(&map_q, q_full, smem + SM::Q + t * SM::TILE + h * SM::HALF, h * 64, c.kh * p.group,
                           c.tok0 + t * tc.per_tile, c.req);
@@ -399,14 +410,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const uint32_t dS = tbase + col_s(t), dO = tbase + col_o(t), dP = tbase + col_p(t);
       int i = 0, g = 0, cs = 0;   // cs: this stream's key tiles in earlier pieces
       bool okw = true;
-      Piece c;
-      for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
-        done(turn);
-        if (c.nk == 0) continue;
+      auto run = [&](const Piece& c) {
         const int n = tiles_of(c, t);
-        const uint64_t dQ = dQ0 + (uint64_t)((c.active == 2 ? t : 0) * (SM::TILE >> 4));
+        const uint64_t dQ = dQ0 + (uint64_t)((HALVES ? 0 : t) * (SM::TILE >> 4));
         auto issue_s = [&](int j) {
-          const int jt = key_tile(c, t, j), st = (g + jt) % ST;
+          const int jt = key_tile(t, j), st = (g + jt) % ST;
           const bool beta = has_beta(tile_of(c, jt));
           if (leader) {
             const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
@@ -418,13 +426,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(st * (XTILE >> 4)), idesc_s, 1);
             umma_commit(&s_full[t]);
             umma_commit(&k_empty[st]);
-            if (c.active == 1) umma_commit(&k_empty[st]);
             if (j == n - 1) umma_commit(q_empty);
           }
           __syncwarp();
         };
         auto issue_o = [&](int j) {
-          const int st = (g + key_tile(c, t, j)) % ST;
+          const int st = (g + key_tile(t, j)) % ST;
           if (leader) {
             const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
@@ -432,14 +439,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               umma_bf16_ts(dO, dP + ks * 8, bv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0));
             umma_commit(&o_done[t]);
             umma_commit(&v_empty[st]);
-            if (c.active == 1) umma_commit(&v_empty[st]);
           }
           __syncwarp();
         };
         // The rows to zero of a key tile, read once its K has landed (the producer
         // reuses the words before its V is used).
         auto rows_out = [&](int j) {
-          const int jt = key_tile(c, t, j);
+          const int jt = key_tile(t, j);
           const Tile kt = tile_of(c, jt);
           return (kt.own ? kt.valid < TM : p.bias != nullptr)
                      ? *reinterpret_cast<const uint4*>(smem + SM::MASK + ((g + jt) % ST) * 16)
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         auto zero_rows = [&](const uint4& m, int base, int j) {
           if (!(m.x | m.y | m.z | m.w)) return;
           uint8_t* tile =
-              smem + base + ((g + key_tile(c, t, j)) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
+              smem + base + ((g + key_tile(t, j)) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
           for (int row = 0; row < TM; ++row) {
             const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
             if ((word >> (row & 31) & 1) && lane < 8 * SM::HALVES)
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           __syncwarp();
         };
         auto wait_tile = [&](uint64_t* bar, int j) {
-          const int gt = g + key_tile(c, t, j);
+          const int gt = g + key_tile(t, j);
           return wait(&bar[gt % ST], gt / ST);
         };
         uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
@@ -495,9 +501,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             scores(j + 1);
           }
         }
+        cs += n;
+      };
+      Piece c;
+      for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+        done(turn);
+        if (c.nk == 0) continue;
+        run(c);
         ++i;
         g += c.nk;
-        cs += n;
       }
     } else {
       // ------------------------------ planner ------------------------------
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       walk.req0 = start_req0;
       Piece c;
       for (uint32_t turn = 0;; ++turn) {
-        const bool more = next_piece(p, tc, walk, c);
+        const bool more = next_piece<HALVES>(p, tc, walk, c);
         if (!wait(&piece_empty[turn % RING], turn / RING + 1)) break;
         if (lane == 0) {
           if (!more) c.req = -1;
@@ -529,14 +541,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int tl = row_i / p.group, head = row_i - tl * p.group;
     int cs = 0, ih = 0;   // ih: pieces in halves so far
     bool okw = true;
-    Piece c;
-    for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+    auto run = [&](const Piece& c) {
       const int n = tiles_of(c, t);
-      const bool halves = c.active == 1 && c.nk > 1;
+      const bool halves = HALVES && c.nk > 1;
       // this thread's row
       Row row;
       {
-        const int tok = c.tok0 + (c.active == 2 ? t : 0) * tc.per_tile + tl;
+        const int tok = c.tok0 + (HALVES ? 0 : t) * tc.per_tile + tl;
         row.h = c.kh * p.group + head;
         row.live = tl < tc.per_tile && tok < c.tok_end;
         row.r = c.req;
@@ -588,7 +599,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
         if (CAUSAL) {   // keys ahead of this row
-          const Tile kt = tile_of(c, key_tile(c, t, j));
+          const Tile kt = tile_of(c, key_tile(t, j));
           if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {
             const int end = limit - kt.key0;
 #pragma unroll
@@ -663,13 +674,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           okw = wait(half_read, ih);
         }
         ++ih;
-        done(turn);
-        continue;
+        return;
       }
-      if (c.active == 1 && t == 1) {
-        done(turn);
-        continue;
-      }
+      if (HALVES && t == 1) return;
       float f0 = 1.f, f1 = 0.f;
       if (halves) {
         okw = okw && wait(half_there, ih);
@@ -684,7 +691,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           m_raw = m;
         }
       }
-      if (!okw || *abort_flag) break;
+      if (!okw || *abort_flag) return;
       const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
       const float inv = some ? 1.0f / l : 0.f;
       const bool direct = c.first && c.last && p.s2 == 0;
@@ -739,6 +746,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             for (int s = c.slot + 1; s < p.s1; ++s) p.ws_ml[s * p.rows + at] = make_float2(-INFINITY, 0.f);
         }
       }
+    };
+    Piece c;
+    for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
+      run(c);
       done(turn);
     }
   }
@@ -780,21 +791,21 @@ bool tc_takes(const Params& p, int head_dim, bool fold) {
 
 // The register split needs a launch with TC_REGS registers per thread; refuse
 // to launch otherwise (it would never start).
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, bool HALVES>
 static int check_regs() {
   cudaFuncAttributes fa;
-  if (cudaFuncGetAttributes(&fa, tc_kernel<D, CAUSAL>) != cudaSuccess)
+  if (cudaFuncGetAttributes(&fa, tc_kernel<D, CAUSAL, HALVES>) != cudaSuccess)
     return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: cudaFuncGetAttributes failed");
   if (fa.numRegs * TC_THREADS < TC_LOW * 128 + TC_HIGH * 256)
     return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: kernel built with %d registers/thread", fa.numRegs);
   return GPA_OK;
 }
 
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, bool HALVES>
 static int launch(const Params& p, const TcPlan& t, cudaStream_t st) {
   static bool checked = false;
   if (!checked) {
-    const int rc = check_regs<D, CAUSAL>();
+    const int rc = check_regs<D, CAUSAL, HALVES>();
     if (rc) return rc;
     checked = true;
   }
@@ -811,15 +822,21 @@ static int launch(const Params& p, const TcPlan& t, cudaStream_t st) {
   if (rc) return rc;
   if (!pre) mkp = mko, mvp = mvo;   // never read
   if (!own) mko = mkp, mvo = mvp;
-  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D>::ALLOC);
+  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D, CAUSAL, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D>::ALLOC);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
-  tc_kernel<D, CAUSAL><<<t.ctas, TC_THREADS, TcSmem<D>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
+  tc_kernel<D, CAUSAL, HALVES><<<t.ctas, TC_THREADS, TcSmem<D>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
   return check_launch("gpa_attention_shared_prefix");
 }
 
+template <int D>
+static int launch_form(const Params& p, const TcPlan& t, cudaStream_t st) {
+  const bool causal = p.causal && !t.fold;
+  if (t.halves) return causal ? launch<D, true, true>(p, t, st) : launch<D, false, true>(p, t, st);
+  return causal ? launch<D, true, false>(p, t, st) : launch<D, false, false>(p, t, st);
+}
+
 int launch_tc(const Params& p, int head_dim, const TcPlan& t, cudaStream_t st) {
-  if (p.causal && !t.fold) return head_dim == 64 ? launch<64, true>(p, t, st) : launch<128, true>(p, t, st);
-  return head_dim == 64 ? launch<64, false>(p, t, st) : launch<128, false>(p, t, st);
+  return head_dim == 64 ? launch_form<64>(p, t, st) : launch_form<128>(p, t, st);
 }
 
 }  // namespace prefix

@@ -25,7 +25,7 @@ constexpr int BN = 64;         // keys per tile
 constexpr int THREADS = 128;
 constexpr int kSlotTiles = 4;  // at least this many tiles per chunk
 constexpr int kSms = 148;
-constexpr int kLeastSteps = 4;  // at least this many steps per CTA of the tensor-core kernel
+constexpr int kLeastSteps = 4;  // the tensor-core kernel cuts no item into parts of fewer steps
 
 template <int D>
 struct Cfg {
@@ -348,14 +348,17 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     const int t = (int)(it % p.rt1);
     it /= p.rt1;
     run_item<D, WM1, false>(p, smem, (int)(it / p.s1), 0, t, (int)(it % p.s1));
-    return;
+  } else {
+    it -= n1;
+    const int t = (int)(it % p.rt2);
+    it /= p.rt2;
+    const int s = (int)(it % p.s2);
+    it /= p.s2;
+    run_item<D, WM2, true>(p, smem, (int)(it % p.kv_heads), (int)(it / p.kv_heads), t, s);
   }
-  it -= n1;
-  const int t = (int)(it % p.rt2);
-  it /= p.rt2;
-  const int s = (int)(it % p.s2);
-  it /= p.s2;
-  run_item<D, WM2, true>(p, smem, (int)(it % p.kv_heads), (int)(it / p.kv_heads), t, s);
+  // Behind tc_kernel this grid starts before that one's end (neither reads what
+  // the other writes); its own end, which the join waits for, must not come first.
+  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the chunks of a row with W warps (1: a warp's own row, 8: the block's).
@@ -433,52 +436,97 @@ __device__ __forceinline__ void join_row(const Params& p, int64_t row, float (*p
   if (p.lse && lane == 0) p.lse[r * p.lse_sr + h * p.lse_sh + m] = l == 0.f ? -INFINITY : mx + log2f(l);
 }
 
-// Whether a row's chunks are to be joined: not past its request's queries, nor
-// written by the tensor-core kernel already.
+// Whether a row's chunks are to be joined: not past its request's queries.
 __device__ __forceinline__ bool to_join(const Params& p, int64_t row) {
   if (row >= p.rows) return false;
-  if (p.q_len) {
-    const uint32_t tok = (uint32_t)row / (uint32_t)p.heads;
-    if ((int)(tok % (uint32_t)p.queries) >= __ldg(p.q_len + tok / (uint32_t)p.queries)) return false;
-  }
-  return p.s1 + p.s2 == 0 || p.ws_ml[row].y != kWritten;
+  if (!p.q_len) return true;
+  const uint32_t tok = (uint32_t)row / (uint32_t)p.heads;
+  return (int)(tok % (uint32_t)p.queries) < __ldg(p.q_len + tok / (uint32_t)p.queries);
 }
 
-// WIDE: a block per row, each warp taking every eighth chunk.  Else RPW rows per
-// warp: most rows of a large call are written already, and a look at RPW of them
-// at once finds the others.  The launch overlaps the end of the kernel before it
-// (a programmatic dependency), which the first line waits for.
-template <int D, bool WIDE, int RPW>
+// Joins rows_kernel's chunks.  WIDE: a block per row, each warp taking every
+// eighth chunk, else a warp per row.  The launch overlaps the end of the kernel
+// before it (a programmatic dependency), which the first line waits for.
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if constexpr (WIDE) {
     __shared__ float part[8][D];
     if (to_join(p, blockIdx.x)) join_row<D, 8>(p, blockIdx.x, part);
   } else {
-    const int lane = threadIdx.x & 31;
-    const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW;
-    unsigned left = __ballot_sync(0xffffffffu, lane < RPW && to_join(p, row0 + lane));
-    for (; left; left &= left - 1) join_row<D, 1>(p, row0 + __ffs(left) - 1, nullptr);
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (to_join(p, row)) join_row<D, 1>(p, row, nullptr);
   }
 }
 
+// Joins tc_kernel's parts (and rows_kernel's chunks of the caches, in a folded
+// call): a thread per row of a 128-row tile, 32 features of it.  Rows whose output
+// is written already leave at once.
 template <int D>
-static int launch_join(const Params& p, cudaStream_t st) {
-  // eight warps per row from where one would go twice through its eight loads,
-  // several rows per warp from where they fill the GPU all the same
-  const bool wide = p.s1 + p.s2 > 16 && p.rows <= 16384, many = !wide && p.rows > 32768;
+__global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const TcPlan tc) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int i = threadIdx.x, block = blockIdx.x, f0 = blockIdx.y * 32;
+  const int rk = block / tc.tiles, req = rk / p.kv_heads, kh = rk - req * p.kv_heads;
+  const Row w = tile_row(p, tc, kh, req, block - rk * tc.tiles, i);
+  if (!w.live) return;
+  const float2* tml = p.tc_ml + (int64_t)block * 128 + i;
+  const int64_t tstep = (int64_t)tc.blocks * 128;
+  const float2 first = tml[0];
+  if (first.y == kWritten) return;
+  const int64_t row = row_index(p, w);
+  const int slots = p.s1 + p.s2;
+  float mx = first.x;
+#pragma unroll 4
+  for (int s = 1; s < tc.slots; ++s) mx = fmaxf(mx, tml[s * tstep].x);
+#pragma unroll 4
+  for (int s = 0; s < slots; ++s) mx = fmaxf(mx, p.ws_ml[s * p.rows + row].x);
+  float l = 0.f, v[32];
+#pragma unroll
+  for (int u = 0; u < 32; ++u) v[u] = 0.f;
+  // one part: its weight, and where it wrote any output, that
+  auto add = [&](const float2 ml, const float4* o, int64_t step) {
+    const float f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
+    l = fmaf(ml.y, f, l);
+    if (f > 0.f) {
+      float4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = o[u * step];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        v[4 * u] = fmaf(f, x[u].x, v[4 * u]);
+        v[4 * u + 1] = fmaf(f, x[u].y, v[4 * u + 1]);
+        v[4 * u + 2] = fmaf(f, x[u].z, v[4 * u + 2]);
+        v[4 * u + 3] = fmaf(f, x[u].w, v[4 * u + 3]);
+      }
+    }
+  };
+  for (int s = 0; s < tc.slots; ++s)
+    add(tml[s * tstep], p.tc_o + (((int64_t)s * tc.blocks + block) * (D / 4) + f0 / 4) * 128 + i, 128);
+  for (int s = 0; s < slots; ++s)
+    add(p.ws_ml[s * p.rows + row], reinterpret_cast<const float4*>(p.ws_o + (s * p.rows + row) * D + f0), 1);
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
+  uint4* dst = reinterpret_cast<uint4*>(p.o + w.r * p.o_sr + w.h * p.o_sh + w.m * p.o_sm + f0);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    dst[u] = make_uint4(pack_bf16x2(v[8 * u] * inv, v[8 * u + 1] * inv), pack_bf16x2(v[8 * u + 2] * inv, v[8 * u + 3] * inv),
+                        pack_bf16x2(v[8 * u + 4] * inv, v[8 * u + 5] * inv), pack_bf16x2(v[8 * u + 6] * inv, v[8 * u + 7] * inv));
+  if (p.lse && f0 == 0) p.lse[w.r * p.lse_sr + w.h * p.lse_sh + w.m] = l == 0.f ? -INFINITY : mx + log2f(l);
+}
+
+// A launch that may begin before the kernel ahead of it in the stream has ended.
+template <typename... P, typename... A>
+static int launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(wide ? p.rows : many ? (p.rows + 127) / 128 : (p.rows + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = wide   ? cudaLaunchKernelEx(&cfg, join_kernel<D, true, 1>, p)
-                        : many ? cudaLaunchKernelEx(&cfg, join_kernel<D, false, 16>, p)
-                               : cudaLaunchKernelEx(&cfg, join_kernel<D, false, 1>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
   return check_launch("gpa_attention_shared_prefix");
 }
@@ -489,11 +537,43 @@ struct Plan {
   int wm1, rt1, s1, wm2, rt2, s2, chunk;
   int64_t items, rows;
   TcPlan tc;
-  int64_t slots() const { return s1 + s2; }
-  int64_t bytes(int head_dim) const { return slots() * rows * (head_dim + 2) * 4; }
+  int64_t floats(int head_dim) const {   // of the partial outputs
+    return (tc_run ? (int64_t)tc.slots * tc.blocks * 128 * (head_dim + 2) : 0) + (s1 + s2) * rows * (head_dim + 2);
+  }
 };
 
 static int warps_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// The tensor-core kernel's share: over prefix and own keys of each request, or
+// folded over the prefix alone.  False where its counts would not fit.
+static bool plan_tc(TcPlan* tc, bool fold, int requests, int queries, int group, int kv_heads, int64_t prefix_tiles,
+                    int64_t cache_tiles, int64_t* total) {
+  const int64_t tokens = fold ? (int64_t)requests * queries : queries;
+  tc->fold = fold;
+  tc->tokens = (int)tokens;
+  tc->per_tile = 128 / group;
+  const int64_t tiles = (tokens + tc->per_tile - 1) / tc->per_tile;
+  const int64_t heads = (int64_t)kv_heads * (fold ? 1 : requests);
+  tc->tiles = (int)tiles;
+  tc->halves = tiles == 1;
+  // The units of all items at full lengths (the kernel counts the real ones), and
+  // what a CTA gets of them.  An item is cut where a span ends, into at most
+  // units / span + 2 parts; twice the units / span leaves room for spans that
+  // shorter lengths make shorter.
+  const int64_t keys = std::max<int64_t>(prefix_tiles + (fold ? 0 : cache_tiles), 1);
+  const int64_t steps = tc->halves ? (keys + 1) / 2 : keys;
+  const int each = tiles > 1 ? kPair : kSingle;
+  const int64_t units = steps * each, least = std::min<int64_t>(kLeastSteps, steps) * each;
+  if ((double)(tiles / 2 * kPair + tiles % 2 * kSingle) * steps * heads >= 1e9 || (double)tiles * heads >= 1e7) return false;
+  *total = (tiles / 2 * kPair + tiles % 2 * kSingle) * steps * heads;
+  const int64_t span = std::max((*total + kSms - 1) / kSms, least);
+  const int64_t cuts = std::min(2 * ((units + span - 1) / span), std::max<int64_t>(units / least, 1));
+  tc->blocks = (int)(tiles * heads);
+  tc->least = (int)std::max((units + cuts - 1) / cuts, least);
+  tc->ctas = (int)std::min<int64_t>(kSms, (*total + least - 1) / least);
+  tc->slots = (int)((units + tc->least - 1) / tc->least) + 1;
+  return true;
+}
 
 // joint, fold: whether the tensor-core kernel can take the call in that form.
 static Plan make_plan(int requests, int queries, int heads, int kv_heads, int head_dim, int prefix, int cache,
@@ -501,45 +581,47 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   Plan p{};
   const int group = heads / kv_heads;
   const int64_t r1 = (int64_t)requests * queries * group, r2 = (int64_t)queries * group;
+  const int64_t t1 = (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
   p.rows = r1 * kv_heads;
-  joint = joint && r2 > 64 && prefix + (int64_t)cache > 0;
-  fold = fold && !joint && r1 > 128 && prefix > 0;
-  p.tc_run = joint || fold;
-  p.rows_run = !joint && !(fold && cache == 0);
-  if (p.tc_run) {
-    p.tc.fold = fold;
-    p.tc.tokens = fold ? requests * queries : queries;
-    p.tc.per_tile = 128 / group;
-    // The units of all items at full lengths (the kernel counts the real ones),
-    // and what a CTA gets of them.  An item is cut where a span ends: into at most
-    // units / span + 2 parts; twice the units / span leaves room for spans that
-    // shorter lengths make shorter.
-    const int64_t tiles = (p.tc.tokens + p.tc.per_tile - 1) / p.tc.per_tile;
-    const int64_t keys = (prefix + 127) / 128 + (fold ? 0 : (cache + 127) / 128);
-    p.tc.halves = tiles == 1;
-    const int64_t steps = p.tc.halves ? (keys + 1) / 2 : keys;
-    const int each = tiles > 1 ? kPair : kSingle;
-    const int64_t units = steps * each, least = kLeastSteps * each;
-    const int64_t total = (tiles / 2 * kPair + tiles % 2 * kSingle) * steps * kv_heads * (fold ? 1 : requests);
-    const int64_t span = std::max((total + kSms - 1) / kSms, least);
-    const int64_t cuts = std::min(2 * ((units + span - 1) / span), std::max<int64_t>(units / least, 1));
-    p.tc.least = (int)std::min<int64_t>(std::max((units + cuts - 1) / cuts, least), 1 << 30);
-    p.tc.ctas = (int)std::min<int64_t>(kSms, (total + least - 1) / least);
-    p.s1 = (int)((units + p.tc.least - 1) / p.tc.least) + 1;
+  // Which kernels: the least time by a model in units of half a microsecond of an
+  // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
+  // 1.2 or 1.6 for 16, 32 or 64 rows (16 heads, 66,845 keys: 57, 74 and 94 us;
+  // mma.sync ends at 0.2-0.25 PFLOP/s); tc_kernel takes kPair or kSingle per step,
+  // or in halves, which wait for HBM, 3.5 (75 us for 64 rows), and 20 to start
+  // and end on every SM.
+  auto rows_cost = [&](int64_t rows, int64_t tiles) {
+    const int wm = warps_for(rows);
+    return (double)((rows + 16 * wm - 1) / (16 * wm)) * tiles * (wm == 1 ? 0.9 : wm == 2 ? 1.2 : 1.6) * kv_heads;
+  };
+  const double own_cost = requests * rows_cost(r2, t2);
+  double least = rows_cost(r1, t1) + own_cost;
+  TcPlan tc{};
+  int64_t total = 0;
+  const int64_t k1 = (prefix + 127) / 128, k2 = (cache + 127) / 128;
+  for (int way = 0; way < 2; ++way) {   // joint, folded
+    if (!(way ? fold && prefix > 0 : joint && prefix + (int64_t)cache > 0)) continue;
+    if (!plan_tc(&tc, way, requests, queries, group, kv_heads, k1, k2, &total)) continue;
+    const double cost = (tc.halves ? total * 3.5 / kSingle : (double)total) + (way ? own_cost : 0) + 20.0 * kSms;
+    if (cost < least) {
+      least = cost;
+      p.tc = tc;
+      p.tc_run = true;
+    }
   }
+  p.rows_run = !p.tc_run || (p.tc.fold && cache > 0);
   if (p.rows_run) {
-    const int64_t t1 = p.tc_run ? 0 : (prefix + BN - 1) / BN, t2 = (cache + BN - 1) / BN;
+    const int64_t tiles1 = p.tc_run ? 0 : t1;
     p.wm1 = p.tc_run ? 4 : warps_for(r1);
     p.wm2 = warps_for(r2);
     p.rt1 = p.tc_run ? 0 : (int)((r1 + p.wm1 * 16 - 1) / (p.wm1 * 16));
     p.rt2 = (int)((r2 + p.wm2 * 16 - 1) / (p.wm2 * 16));
-    const int64_t units = kv_heads * (p.rt1 * t1 + (int64_t)requests * p.rt2 * t2);
+    const int64_t units = kv_heads * (p.rt1 * tiles1 + (int64_t)requests * p.rt2 * t2);
     // two items per resident CTA: short enough to even out requests of unequal
     // lengths, long enough that the partial outputs are a small share
-    const int64_t want = 148ll * (head_dim == 64 ? 3 : 2) * 2;
+    const int64_t want = (int64_t)kSms * (head_dim == 64 ? 3 : 2) * 2;
     const int64_t per = std::max<int64_t>((units + want - 1) / want, kSlotTiles);
     p.chunk = (int)std::min<int64_t>(per, 1 << 24) * BN;
-    if (!p.tc_run) p.s1 = (int)((t1 + per - 1) / per);
+    p.s1 = (int)((tiles1 + per - 1) / per);
     p.s2 = (int)((t2 + per - 1) / per);
     p.items = kv_heads * ((int64_t)p.rt1 * p.s1 + (int64_t)requests * p.rt2 * p.s2);
   }
@@ -547,9 +629,10 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
 }
 
 template <int D, int WM1, int WM2>
-static int launch_rows(const Params& p, int64_t items, cudaStream_t st) {
+static int launch_rows(const Params& p, int64_t items, bool early, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, WM1, WM2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
+  if (early) return launch_early(rows_kernel<D, WM1, WM2>, dim3((unsigned)items), THREADS, Cfg<D>::SMEM, st, p);
   rows_kernel<D, WM1, WM2><<<(unsigned)items, THREADS, Cfg<D>::SMEM, st>>>(p);
   return check_launch("gpa_attention_shared_prefix");
 }
@@ -557,19 +640,24 @@ static int launch_rows(const Params& p, int64_t items, cudaStream_t st) {
 template <int D>
 static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
   int rc = GPA_OK;
-  if (plan.tc_run) rc = launch_tc(p, D, plan.tc, st);
+  const bool tc = plan.tc_run;
+  if (tc) rc = launch_tc(p, D, plan.tc, st);
   if (!rc && plan.rows_run && plan.items > 0) {
     switch (plan.wm1 * 8 + plan.wm2) {   // wm2 <= wm1: own rows are part of the prefix's
-      case 1 * 8 + 1: rc = launch_rows<D, 1, 1>(p, plan.items, st); break;
-      case 2 * 8 + 1: rc = launch_rows<D, 2, 1>(p, plan.items, st); break;
-      case 2 * 8 + 2: rc = launch_rows<D, 2, 2>(p, plan.items, st); break;
-      case 4 * 8 + 1: rc = launch_rows<D, 4, 1>(p, plan.items, st); break;
-      case 4 * 8 + 2: rc = launch_rows<D, 4, 2>(p, plan.items, st); break;
-      default: rc = launch_rows<D, 4, 4>(p, plan.items, st); break;
+      case 1 * 8 + 1: rc = launch_rows<D, 1, 1>(p, plan.items, tc, st); break;
+      case 2 * 8 + 1: rc = launch_rows<D, 2, 1>(p, plan.items, tc, st); break;
+      case 2 * 8 + 2: rc = launch_rows<D, 2, 2>(p, plan.items, tc, st); break;
+      case 4 * 8 + 1: rc = launch_rows<D, 4, 1>(p, plan.items, tc, st); break;
+      case 4 * 8 + 2: rc = launch_rows<D, 4, 2>(p, plan.items, tc, st); break;
+      default: rc = launch_rows<D, 4, 4>(p, plan.items, tc, st); break;
     }
   }
   if (rc) return rc;
-  return launch_join<D>(p, st);
+  if (tc) return launch_early(join_tiles_kernel<D>, dim3(plan.tc.blocks, D / 32), 128, 0, st, p, plan.tc);
+  // eight warps per row from where one would go twice through its eight loads
+  if (p.s1 + p.s2 > 16 && p.rows <= 16384)
+    return launch_early(join_kernel<D, true>, dim3((unsigned)p.rows), 256, 0, st, p);
+  return launch_early(join_kernel<D, false>, dim3((unsigned)((p.rows + 7) / 8)), 256, 0, st, p);
 }
 
 static int check_sizes(const char* what, int requests, int queries, int heads, int kv_heads, int head_dim, int prefix,
@@ -596,9 +684,9 @@ extern "C" int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int
   if (requests == 0 || queries == 0) return 0;
   // strides decide which kernels can run: room for each way
   int64_t bytes = 0;
-  for (int way = 0; way < 3; ++way)
-    bytes = std::max(bytes, prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache, way == 1,
-                                              way == 2).bytes(head_dim));
+  for (int way = 0; way < 4; ++way)
+    bytes = std::max(bytes, 4 * prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache, way & 1,
+                                                  way & 2).floats(head_dim));
   return bytes;
 }
 
@@ -655,14 +743,18 @@ extern "C" int gpa_attention_shared_prefix(
                         prefix::tc_takes(p, head_dim, false), prefix::tc_takes(p, head_dim, true));
   if (plan.items >= (1ll << 31))
     return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
-  const int64_t bytes = plan.bytes(head_dim);
+  const int64_t bytes = 4 * plan.floats(head_dim);
   if (bytes && (!workspace || !aligned16(workspace) || workspace_bytes < bytes))
     return fail(GPA_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
   p.status = status;
   p.rt1 = plan.rt1; p.s1 = plan.s1; p.rt2 = plan.rt2; p.s2 = plan.s2; p.chunk = plan.chunk;
   p.rows = plan.rows;
-  p.ws_o = (float*)workspace;
-  p.ws_ml = reinterpret_cast<float2*>(p.ws_o + plan.slots() * plan.rows * head_dim);
+  // the tiles' outputs (whole lines each), the rows', then their maxima and sums
+  const int64_t tile_rows = plan.tc_run ? (int64_t)plan.tc.slots * plan.tc.blocks * 128 : 0;
+  p.tc_o = (float4*)workspace;
+  p.ws_o = (float*)workspace + tile_rows * head_dim;
+  p.tc_ml = reinterpret_cast<float2*>(p.ws_o + (plan.s1 + plan.s2) * plan.rows * head_dim);
+  p.ws_ml = p.tc_ml + tile_rows;
   cudaStream_t st = (cudaStream_t)stream;
   return head_dim == 64 ? prefix::launch<64>(p, plan, st) : prefix::launch<128>(p, plan, st);
 }

@@ -25,6 +25,10 @@ struct Params {
   int64_t rows;                  // requests * queries * heads
   float* ws_o;                   // [s1 + s2][rows][D]
   float2* ws_ml;                 // [s1 + s2][rows]: maximum (log2 units) and sum
+  // tc_kernel's: a row tile's outputs lie feature group by feature group, so that
+  // its threads, one per row, write and read whole lines
+  float4* tc_o;                  // [slots][blocks][D / 4][128 rows]
+  float2* tc_ml;                 // [slots][blocks][128 rows]
   int* status;
 };
 
@@ -48,19 +52,39 @@ __device__ __forceinline__ int query_count(const Params& p, int r) {
 // What the sum of a row's first partial output holds when its output is written.
 constexpr float kWritten = -1.0f;
 
-// Units of time that a step of it counts, with rows in two tiles or in one.
+// Units of time that a step of tc_kernel counts, with rows in two tiles or in one.
 constexpr int kPair = 3, kSingle = 2;
 
-// The tensor-core kernel's share of a call: 2 x 128-row tiles over the prefix
-// and, unless `fold`, each request's own keys.
+// The tensor-core kernel's share of a call: 128-row tiles over the prefix and,
+// unless `fold`, each request's own keys.
 struct TcPlan {
   int fold;      // rows run through all requests (prefix only), else within one request
   int tokens;    // tokens a tile's rows may come from: requests * queries (fold) or queries
   int per_tile;  // tokens of a 128-row tile
+  int tiles;     // of the tokens
+  int blocks;    // tiles of all key heads (and requests)
   int halves;    // every item has rows in one tile only
   int ctas;      // each takes a span of the units of work
-  int least;     // of at least so many: no item is cut into more than s1 parts
+  int least;     // of at least so many: no item is cut into more than `slots` parts
+  int slots;
 };
+
+// Row i of row tile `block` of tc_kernel.
+__device__ __forceinline__ Row tile_row(const Params& p, const TcPlan& tc, int kh, int req, int tile, int i) {
+  Row w;
+  const int tl = i / p.group, tok = tile * tc.per_tile + tl;
+  w.h = kh * p.group + (i - tl * p.group);
+  w.live = tl < tc.per_tile && tok < tc.tokens;
+  w.r = req;
+  w.m = tok;
+  if (tc.fold) {
+    w.r = tok / p.queries;
+    w.m = tok - w.r * p.queries;
+  }
+  if (w.live && p.q_len) w.live = w.m < __ldg(p.q_len + w.r);
+  return w;
+}
+
 // Whether the kernel can take the call's strides and scale.
 bool tc_takes(const Params& p, int head_dim, bool fold);
 int launch_tc(const Params& p, int head_dim, const TcPlan& t, cudaStream_t st);

@@ -44,14 +44,17 @@ static_assert(TC_LOW * 128 + TC_HIGH * 256 <= TC_REGS * TC_THREADS, "register sp
 
 constexpr int RING = 4;   // pieces handed on ahead
 
-template <int D>
+template <int D, bool HALVES>
 struct TcSmem {
-  static constexpr int HALVES = D / 64;          // a row is HALVES swizzled rows of 128 bytes
-  static constexpr int HALF = TM * 128;          // 16 KB
-  static constexpr int TILE = HALVES * HALF;
-  static constexpr int STAGES = D == 64 ? 3 : 2;
-  static constexpr int Q = 0;                    // 2 tiles
-  static constexpr int K = Q + 2 * TILE;
+  static constexpr int ATOMS = D / 64;           // a row is ATOMS swizzled rows of 128 bytes
+  static constexpr int ATOM = TM * 128;          // 16 KB
+  static constexpr int TILE = ATOMS * ATOM;
+  // In halves each stage belongs to one stream (an even number of them): an issuer
+  // sees every phase of the barriers that it waits on.
+  static constexpr int STAGES = D == 64 ? (HALVES ? 4 : 3) : 2;
+  static_assert(!HALVES || STAGES % 2 == 0, "stages of the two streams");
+  static constexpr int Q = 0;                    // 1 or 2 tiles
+  static constexpr int K = Q + (HALVES ? 1 : 2) * TILE;
   static constexpr int V = K + STAGES * TILE;
   static constexpr int ONES = V + STAGES * TILE;
   static constexpr int BETA = ONES + XTILE;
@@ -95,7 +98,7 @@ struct Load {
   int pairs2;      // pairs with two row tiles
   bool single;     // and one with one
   int steps;       // of a pair (no keys at all count as one, to write the empty rows)
-  int64_t head;    // units of one key head
+  int head;        // units of one key head
 };
 template <bool HALVES>
 __device__ __forceinline__ Load load_of(const Params& p, const TcPlan& tc, int r) {
@@ -106,22 +109,22 @@ __device__ __forceinline__ Load load_of(const Params& p, const TcPlan& tc, int r
   w.single = tiles & 1;
   const int keys = max(1, (p.prefix + TM - 1) / TM + (tc.fold ? 0 : (own_length(p, r) + TM - 1) / TM));
   w.steps = HALVES ? (keys + 1) >> 1 : keys;
-  w.head = (int64_t)w.steps * (kPair * w.pairs2 + (w.single ? kSingle : 0));
+  w.head = w.steps * (kPair * w.pairs2 + (w.single ? kSingle : 0));
   return w;
 }
 
 // A CTA's share of one item.
 struct Piece {
-  int req, kh, tok0, tok_end;
+  int req, kh, tile;   // the first of its two row tiles
   int len, qlen;
   int j0, nk;        // key tiles (nk may be 0: nothing to see here)
   int slot;          // which partial output
   bool first, last;  // holds the item's first, last step
 };
 struct Walk {
-  int64_t pos, end, span;   // this CTA's units
+  int pos, end, span;   // this CTA's units (all of a call's fit 31 bits)
   int req;
-  int64_t req0;             // first unit of the request
+  int req0;             // first unit of the request
 };
 template <bool HALVES>
 __device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Walk& w, Piece& c) {
@@ -133,28 +136,27 @@ __device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Wa
       w.req0 += ld.head * p.kv_heads;
       ld = load_of<HALVES>(p, tc, ++w.req);
     }
-    const int64_t x = w.pos - w.req0;
-    c.kh = (int)(x / ld.head);
-    const int64_t y = x - c.kh * ld.head;
+    const int x = w.pos - w.req0;
+    c.kh = x / ld.head;
+    const int y = x - c.kh * ld.head;
     steps = ld.steps;
-    const int pair = (int)min(y / (kPair * (int64_t)steps), (int64_t)ld.pairs2);
-    const int64_t at = y - pair * (kPair * (int64_t)steps);   // units of the pair that others have
+    const int pair = min(y / (kPair * steps), ld.pairs2);
+    const int at = y - pair * (kPair * steps);   // units of the pair that others have
     const int each = pair < ld.pairs2 ? kPair : kSingle;
-    const int64_t units = min((int64_t)steps * each - at, w.end - w.pos);
+    const int units = min(steps * each - at, w.end - w.pos);
     // a step goes to the CTA that has its first unit
-    a = (int)((at + each - 1) / each);
-    b = (int)((at + units + each - 1) / each);
-    c.slot = (int)(blockIdx.x - (w.pos - at) / w.span);
-    c.tok0 = pair * 2 * tc.per_tile;
+    a = (at + each - 1) / each;
+    b = (at + units + each - 1) / each;
+    c.slot = blockIdx.x - (w.pos - at) / w.span;
+    c.tile = pair * 2;
     w.pos += units;
   } while (a == b);   // the rest of a step that the CTA before has done
   c.req = w.req;
   c.qlen = tc.fold ? p.queries : query_count(p, c.req);
-  c.tok_end = tc.fold ? tc.tokens : c.qlen;
   c.len = tc.fold ? 0 : own_length(p, c.req);
   // with an order, no row of this pair sees an own key from here on
   const int own_end =
-      p.causal ? min(c.len, max(0, c.len - c.qlen + min(c.tok0 + 2 * tc.per_tile, c.qlen))) : c.len;
+      p.causal ? min(c.len, max(0, c.len - c.qlen + min((c.tile + 2) * tc.per_tile, c.qlen))) : c.len;
   const int tiles = (p.prefix + TM - 1) / TM + (own_end + TM - 1) / TM, each = HALVES ? 2 : 1;
   c.j0 = a * each;
   c.nk = max(0, min(tiles, b * each) - c.j0);
@@ -169,54 +171,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kp,
               const __grid_constant__ CUtensorMap map_vp, const __grid_constant__ CUtensorMap map_ko,
               const __grid_constant__ CUtensorMap map_vo, const Params p, const TcPlan tc) {
-  using SM = TcSmem<D>;
+  using SM = TcSmem<D, HALVES>;
   constexpr int ST = SM::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ int64_t warp_units[TC_THREADS / 32];
-  __shared__ int64_t start_req0;
-  __shared__ int start_req;
+  __shared__ int warp_units[TC_THREADS / 32];
+  __shared__ int start_req0, start_req;
   __shared__ Piece ring[RING];
   asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
   const int warp = warp_id(), lane = lane_id();
-
-  // All units, this CTA's span of them, and the request that it starts in: each
-  // thread adds up a run of requests.
-  Walk walk;
-  {
-    const int nreq = tc.fold ? 1 : p.requests;
-    const int run = (nreq + TC_THREADS - 1) / TC_THREADS;
-    const int r0 = threadIdx.x * run, r1 = min(nreq, r0 + run);
-    int64_t mine = 0;
-    for (int r = r0; r < r1; ++r) mine += load_of<HALVES>(p, tc, r).head * p.kv_heads;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) warp_units[warp] = upto;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int i = 0; i < TC_THREADS / 32; ++i) {
-      if (i < warp) before += warp_units[i];
-      total += warp_units[i];
-    }
-    walk.span = max((total + gridDim.x - 1) / gridDim.x, (int64_t)tc.least);
-    walk.pos = blockIdx.x * walk.span;
-    walk.end = min(total, walk.pos + walk.span);
-    if (walk.pos >= total) return;   // the whole CTA
-    int64_t at = before + upto - mine;
-    if (walk.pos >= at && walk.pos < at + mine) {
-      int r = r0;
-      for (;; ++r) {
-        const int64_t n = load_of<HALVES>(p, tc, r).head * p.kv_heads;
-        if (walk.pos < at + n) break;
-        at += n;
-      }
-      start_req = r;
-      start_req0 = at;
-    }
-  }
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + SM::BARS);
@@ -235,6 +197,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* piece_empty = piece_full + RING;   // RING
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_empty + RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  // All units, this CTA's span of them, and the request that it starts in: each
+  // thread adds up a run of requests.
+  Walk walk;
+  const int nreq = tc.fold ? 1 : p.requests;
+  const int run = (nreq + TC_THREADS - 1) / TC_THREADS;
+  const int r0 = threadIdx.x * run, r1 = min(nreq, r0 + run);
+  int mine = 0;
+  for (int r = r0; r < r1; ++r) mine += load_of<HALVES>(p, tc, r).head * p.kv_heads;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_units[warp] = upto;
 
   // Every barrier's phases run on through the CTA's pieces: per role, `g` counts
   // the key tiles of all pieces so far, `c` those of one stream, `i` the pieces
@@ -267,10 +245,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_kp);
+    tma_prefetch_desc(&map_vp);
+    tma_prefetch_desc(&map_ko);
+    tma_prefetch_desc(&map_vo);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
+  {
+    int before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < TC_THREADS / 32; ++i) {
+      if (i < warp) before += warp_units[i];
+      total += warp_units[i];
+    }
+    walk.span = max((int)((total + gridDim.x - 1) / gridDim.x), tc.least);
+    walk.pos = min((int64_t)blockIdx.x * walk.span, (int64_t)total);
+    walk.end = min((int64_t)walk.pos + walk.span, (int64_t)total);
+    int at = before + upto - mine;
+    if (walk.pos >= at && walk.pos < at + mine) {
+      int r = r0;
+      for (;; ++r) {
+        const int n = load_of<HALVES>(p, tc, r).head * p.kv_heads;
+        if (walk.pos < at + n) break;
+        at += n;
+      }
+      start_req = r;
+      start_req0 = at;
+    }
+    __syncthreads();
+  }
   const int tp = (p.prefix + TM - 1) / TM;
   auto wait = [&](uint64_t* bar, uint32_t phase) {   // the whole warp, bounded
     return __all_sync(0xffffffffu, wait_bar(bar, phase & 1, abort_flag, p.status, kDevTimeout)) != 0;
@@ -300,9 +308,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     return t;
   };
   auto has_beta = [&](const Tile& t) { return t.valid < TM || (!t.own && p.bias != nullptr); };
-  // key tiles of stream t, and which they are
-  auto tiles_of = [](const Piece& c, int t) { return HALVES ? (c.nk - t + 1) >> 1 : c.nk; };
-  auto key_tile = [](int t, int j) { return HALVES ? 2 * j + t : j; };
+  // key tiles of stream t, and which they are (g: all earlier pieces' key tiles)
+  auto tiles_of = [](const Piece& c, int t, int g) { return HALVES ? (c.nk - ((t - g) & 1) + 1) >> 1 : c.nk; };
+  auto key_tile = [](int t, int j, int g) { return HALVES ? 2 * j + ((t - g) & 1) : j; };
   // TMEM columns of a stream
   auto col_s = [](int t) { return (uint32_t)(t * TM); };
   auto col_o = [](int t) { return (uint32_t)(256 + t * D); };
@@ -328,11 +336,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (i > 0 && !(okw = wait(q_empty, i - 1))) break;
         if (lane == 0) {
           constexpr int TILES = HALVES ? 1 : 2;   // past the last token the copy fills with zeros
-          bar_expect_tx(q_full, TILES * SM::HALVES * p.group * tc.per_tile * 128);
+          bar_expect_tx(q_full, TILES * SM::ATOMS * p.group * tc.per_tile * 128);
           for (int t = 0; t < TILES; ++t)
-            for (int h = 0; h < SM::HALVES; ++h)
-              tma_load_4d(&map_q, q_full, smem + SM::Q + t * SM::TILE + h * SM::HALF, h * 64, c.kh * p.group,
-                          c.tok0 + t * tc.per_tile, c.req);
+            for (int h = 0; h < SM::ATOMS; ++h)
+              tma_load_4d(&map_q, q_full, smem + SM::Q + t * SM::TILE + h * SM::ATOM, h * 64, c.kh * p.group,
+                          (c.tile + t) * tc.per_tile, c.req);
         }
         ++i;
         const float* brow = p.bias ? p.bias + c.kh * p.bias_sh : nullptr;
@@ -375,16 +383,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           load_bias(j + 1);
           if (lane == 0) {
             bar_expect_tx(&k_full[s], SM::TILE);
-            for (int h = 0; h < SM::HALVES; ++h)
-              tma_load_4d(t.own ? &map_ko : &map_kp, &k_full[s], smem + SM::K + s * SM::TILE + h * SM::HALF, h * 64,
+            for (int h = 0; h < SM::ATOMS; ++h)
+              tma_load_4d(t.own ? &map_ko : &map_kp, &k_full[s], smem + SM::K + s * SM::TILE + h * SM::ATOM, h * 64,
                           t.key0, c.kh, t.own ? c.req : 0);
           }
           ++gk;
           if (!(okw = wait(&v_empty[s], ph + 1))) break;
           if (lane == 0) {
             bar_expect_tx(&v_full[s], SM::TILE);
-            for (int h = 0; h < SM::HALVES; ++h)
-              tma_load_4d(t.own ? &map_vo : &map_vp, &v_full[s], smem + SM::V + s * SM::TILE + h * SM::HALF, h * 64,
+            for (int h = 0; h < SM::ATOMS; ++h)
+              tma_load_4d(t.own ? &map_vo : &map_vp, &v_full[s], smem + SM::V + s * SM::TILE + h * SM::ATOM, h * 64,
                           t.key0, c.kh, t.own ? c.req : 0);
           }
           ++gv;
@@ -404,23 +412,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       constexpr uint32_t idesc_o = idesc_bf16(TM, D, false, true);
       const uint64_t dQ0 = sdesc_sw128(smem_u32(smem + SM::Q), 16, 1024);
       const uint64_t dK = sdesc_sw128(smem_u32(smem + SM::K), 16, 1024);
-      const uint64_t dV = sdesc_sw128(smem_u32(smem + SM::V), SM::HALF, 1024);
+      const uint64_t dV = sdesc_sw128(smem_u32(smem + SM::V), SM::ATOM, 1024);
       const uint64_t dOnes = sdesc_plain(smem_u32(smem + SM::ONES));
       const uint64_t dBeta = sdesc_plain(smem_u32(smem + SM::BETA));
       const uint32_t dS = tbase + col_s(t), dO = tbase + col_o(t), dP = tbase + col_p(t);
       int i = 0, g = 0, cs = 0;   // cs: this stream's key tiles in earlier pieces
       bool okw = true;
       auto run = [&](const Piece& c) {
-        const int n = tiles_of(c, t);
+        const int n = tiles_of(c, t, g);
         const uint64_t dQ = dQ0 + (uint64_t)((HALVES ? 0 : t) * (SM::TILE >> 4));
         auto issue_s = [&](int j) {
-          const int jt = key_tile(t, j), st = (g + jt) % ST;
+          const int jt = key_tile(t, j, g), st = (g + jt) % ST;
           const bool beta = has_beta(tile_of(c, jt));
           if (leader) {
             const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint64_t off = (uint64_t)((k >> 2) * (SM::HALF >> 4) + (k & 3) * 2);
+              const uint64_t off = (uint64_t)((k >> 2) * (SM::ATOM >> 4) + (k & 3) * 2);
               umma_bf16(dS, dQ + off, bk + off, idesc_s, k != 0);
             }
             if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(st * (XTILE >> 4)), idesc_s, 1);
@@ -431,7 +439,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           __syncwarp();
         };
         auto issue_o = [&](int j) {
-          const int st = (g + key_tile(t, j)) % ST;
+          const int st = (g + key_tile(t, j, g)) % ST;
           if (leader) {
             const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
@@ -445,7 +453,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         // The rows to zero of a key tile, read once its K has landed (the producer
         // reuses the words before its V is used).
         auto rows_out = [&](int j) {
-          const int jt = key_tile(t, j);
+          const int jt = key_tile(t, j, g);
           const Tile kt = tile_of(c, jt);
           return (kt.own ? kt.valid < TM : p.bias != nullptr)
                      ? *reinterpret_cast<const uint4*>(smem + SM::MASK + ((g + jt) % ST) * 16)
@@ -455,17 +463,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         auto zero_rows = [&](const uint4& m, int base, int j) {
           if (!(m.x | m.y | m.z | m.w)) return;
           uint8_t* tile =
-              smem + base + ((g + key_tile(t, j)) % ST) * SM::TILE + (lane >> 3) * SM::HALF + (lane & 7) * 16;
+              smem + base + ((g + key_tile(t, j, g)) % ST) * SM::TILE + (lane >> 3) * SM::ATOM + (lane & 7) * 16;
           for (int row = 0; row < TM; ++row) {
             const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
-            if ((word >> (row & 31) & 1) && lane < 8 * SM::HALVES)
+            if ((word >> (row & 31) & 1) && lane < 8 * SM::ATOMS)
               *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_async_smem();
           __syncwarp();
         };
         auto wait_tile = [&](uint64_t* bar, int j) {
-          const int gt = g + key_tile(t, j);
+          const int gt = g + key_tile(t, j, g);
           return wait(&bar[gt % ST], gt / ST);
         };
         uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
@@ -538,26 +546,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     float2* half_ml = reinterpret_cast<float2*>(smem + SM::ML) + row_i;
     const float c2 = p.scale_log2;
     constexpr float kNoMax = -3.0e38f;   // no key yet
-    const int tl = row_i / p.group, head = row_i - tl * p.group;
-    int cs = 0, ih = 0;   // ih: pieces in halves so far
+    int cs = 0, g = 0, ih = 0;   // ih: pieces in halves so far
     bool okw = true;
     auto run = [&](const Piece& c) {
-      const int n = tiles_of(c, t);
-      const bool halves = HALVES && c.nk > 1;
-      // this thread's row
-      Row row;
-      {
-        const int tok = c.tok0 + (HALVES ? 0 : t) * tc.per_tile + tl;
-        row.h = c.kh * p.group + head;
-        row.live = tl < tc.per_tile && tok < c.tok_end;
-        row.r = c.req;
-        row.m = tok;
-        if (tc.fold) {
-          row.r = tok / p.queries;
-          row.m = tok - row.r * p.queries;
-          if (row.live && p.q_len) row.live = row.m < __ldg(p.q_len + row.r);
-        }
-      }
+      const int n = tiles_of(c, t, g);
+      const bool halves = HALVES && c.nk > 0, other = halves && tiles_of(c, 1, g) > 0;
+      const Row row = tile_row(p, tc, c.kh, c.req, c.tile + (HALVES ? 0 : t), row_i);
       const bool idle = !__any_sync(0xffffffffu, row.live);   // a warp without rows only keeps the barriers going
       // own keys that this row sees end here
       const int limit = CAUSAL ? c.len - c.qlen + row.m + 1 : 0;
@@ -565,8 +559,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       float neg_mc = 0.f;                  // -c2 * m_raw
       auto quarter = [&](float* xq, float neg, float* acc, uint32_t* pk) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float* xg = xq + g * 8;
+        for (int e8 = 0; e8 < 4; ++e8) {
+          float* xg = xq + e8 * 8;
 #pragma unroll
           for (int i = 0; i < 8; i += 2) ffma2(xg[i], xg[i + 1], xg[i], xg[i + 1], c2, c2, neg, neg);
           float e[8];
@@ -574,13 +568,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 8; i += 2) fadd2(acc[i], acc[i + 1], acc[i], acc[i + 1], e[i], e[i + 1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pk[g * 4 + i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+          for (int i = 0; i < 4; ++i) pk[e8 * 4 + i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
         }
       };
       if (idle) {
         for (int j = 0; j < n; ++j) {
-          // the next S may be there before the other warps' P: no second arrival in one phase
-          okw = wait(&s_full[t], cs + j) && (cs + j == 0 || wait(&p_full[t], cs + j - 1));
+          // The next S may be there before the issuer has taken this P: its product
+          // must be done, or the issuer could miss a phase of p_full.
+          okw = wait(&s_full[t], cs + j) && (cs + j == 0 || wait(&o_done[t], cs + j - 1));
           if (!okw) break;
           if (lane == 0) {
             if (D == 64) bar_arrive(&s_empty[t]);
@@ -599,7 +594,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
         if (CAUSAL) {   // keys ahead of this row
-          const Tile kt = tile_of(c, key_tile(t, j));
+          const Tile kt = tile_of(c, key_tile(t, j, g));
           if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {
             const int end = limit - kt.key0;
 #pragma unroll
@@ -663,6 +658,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (lane == 0) bar_arrive(&p_full[t]);
       }
       cs += n;
+      g += c.nk;
       if (okw && n > 0) okw = wait(&o_done[t], cs - 1);
       tc_fence_after();
       if (halves && t == 1) {   // hand over this half: O stays in TMEM until it is read
@@ -683,11 +679,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         ++ih;
         if (okw) {
           tc_fence_after();
-          const float2 other = *half_ml;
-          const float m = fmaxf(m_raw, other.x);
+          const float2 ml = *half_ml;
+          const float m = fmaxf(m_raw, ml.x);
           f0 = fast_exp2((m_raw - m) * c2);
-          f1 = fast_exp2((other.x - m) * c2);
-          l = l * f0 + other.y * f1;
+          f1 = fast_exp2((ml.x - m) * c2);
+          l = l * f0 + ml.y * f1;
           m_raw = m;
         }
       }
@@ -695,7 +691,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
       const float inv = some ? 1.0f / l : 0.f;
       const bool direct = c.first && c.last && p.s2 == 0;
-      const int64_t at = row_index(p, row), to = c.slot * p.rows + at;
+      // the row tile among the partial outputs, and in this piece's slot
+      const int block = (c.req * p.kv_heads + c.kh) * tc.tiles + c.tile + (HALVES ? 0 : t);
+      const int64_t to = (int64_t)c.slot * tc.blocks + block;
       __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
       if (!idle) {
 #pragma unroll
@@ -709,7 +707,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = n > 0 ? __uint_as_float(ov[i]) : 0.f;
-            if (halves) {
+            if (other) {
               tmem_ld32(tbase + lane_off + col_o(1) + u * 32, ov);
               tmem_wait_ld();
 #pragma unroll
@@ -725,9 +723,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             for (int i = 0; i < 4; ++i)
               reinterpret_cast<uint4*>(orow + u * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           } else if (some) {
-            float4* w = reinterpret_cast<float4*>(p.ws_o + to * D + u * 32);
+            float4* w = p.tc_o + (to * (D / 4) + u * 8) * TM + row_i;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            for (int i = 0; i < 8; ++i) w[i * TM] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         }
       }
@@ -739,11 +737,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (row.live) {
         if (direct) {
           if (p.lse) p.lse[row.r * p.lse_sr + row.h * p.lse_sh + row.m] = some ? m_raw * c2 + log2f(l) : -INFINITY;
-          p.ws_ml[at] = make_float2(0.f, kWritten);
+          p.tc_ml[(int64_t)block * TM + row_i] = make_float2(0.f, kWritten);
         } else {
-          p.ws_ml[to] = some ? make_float2(m_raw * c2, l) : make_float2(-INFINITY, 0.f);
+          p.tc_ml[to * TM + row_i] = some ? make_float2(m_raw * c2, l) : make_float2(-INFINITY, 0.f);
           if (c.last)   // slots that no piece of this item takes
-            for (int s = c.slot + 1; s < p.s1; ++s) p.ws_ml[s * p.rows + at] = make_float2(-INFINITY, 0.f);
+            for (int s = c.slot + 1; s < tc.slots; ++s)
+              p.tc_ml[((int64_t)s * tc.blocks + block) * TM + row_i] = make_float2(-INFINITY, 0.f);
         }
       }
     };
@@ -822,9 +821,9 @@ static int launch(const Params& p, const TcPlan& t, cudaStream_t st) {
   if (rc) return rc;
   if (!pre) mkp = mko, mvp = mvo;   // never read
   if (!own) mko = mkp, mvo = mvp;
-  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D, CAUSAL, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D>::ALLOC);
+  cudaError_t e = cudaFuncSetAttribute(tc_kernel<D, CAUSAL, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<D, HALVES>::ALLOC);
   if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "gpa_attention_shared_prefix: %s", cudaGetErrorString(e));
-  tc_kernel<D, CAUSAL, HALVES><<<t.ctas, TC_THREADS, TcSmem<D>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
+  tc_kernel<D, CAUSAL, HALVES><<<t.ctas, TC_THREADS, TcSmem<D, HALVES>::ALLOC, st>>>(mq, mkp, mvp, mko, mvo, p, t);
   return check_launch("gpa_attention_shared_prefix");
 }
 

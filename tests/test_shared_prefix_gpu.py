@@ -376,6 +376,52 @@ def test_many_chunks():
     check(make(1, 130, 1, 1, 128, 20001, 9000, causal=True))
 
 
+@pytest.mark.parametrize("size", [
+    (16, 17, 8, 8, 64, 9000, 90),       # folded: a pair of row tiles and one alone per head
+    (16, 17, 8, 8, 128, 9000, 90),
+    (100, 1, 16, 16, 64, 9000, 33),     # folded: one row tile, its keys in halves
+    (30, 2, 16, 8, 128, 12000, 100),
+    (2, 128, 8, 8, 64, 5000, 300),      # joint: one row tile each, in halves
+    (3, 100, 4, 4, 128, 7000, 200),
+    (5, 300, 4, 4, 64, 3000, 500),      # joint: pairs and one alone
+    (3, 43, 6, 2, 64, 3000, 129),       # 126 rows a tile
+    (1, 2000, 2, 1, 128, 1500, 1000),
+])
+def test_every_form_of_the_kernels(size):
+    """Long enough for the tensor cores: items cut over many CTAs, odd tiles at the
+    end, lengths and orders that leave parts of them empty."""
+    R, M, N = size[0], size[1], size[6]
+    g = torch.Generator().manual_seed(sum(size))
+    lens = torch.randint(0, N + 1, (R,), generator=g).tolist()
+    qs = torch.randint(0, M + 1, (R,), generator=g).tolist()
+    check(make(*size, bias="key"))
+    check(make(*size, own_len=lens, causal=True, seed=1))
+    check(make(*size, bias="head", own_len=lens, q_len=qs, causal=bool(size[0] % 2), seed=2))
+    a = make(*size, bias="key", own_len=[0] * R, seed=3)
+    a["bias"][::5] = -INF
+    a["k_prefix"][:, ::5] = float("nan")
+    a["v_prefix"][:, ::5] = INF
+    check(a)
+
+
+def test_drawn_sizes():
+    g = torch.Generator().manual_seed(77)
+
+    def draw(lo, hi):
+        return int(round(math.exp(float(torch.rand((), generator=g)) * math.log(hi / lo) + math.log(lo))))
+    for i in range(40):
+        H, Hk = [(4, 4), (8, 2), (6, 3), (5, 1)][int(torch.randint(4, (), generator=g))]
+        R, M = draw(1, 40), draw(1, 400)
+        P, N = draw(1, 6000), draw(1, 900)
+        while R * M * H * (P + N) > 60_000_000:
+            R, M = max(1, R // 2), max(1, M * 2 // 3)
+            P = max(1, P // 2)
+        lens = torch.randint(0, N + 1, (R,), generator=g).tolist()
+        check(make(R, M, H, Hk, (64, 128)[i % 2], P, N, bias=(None, "key", "head")[i % 3], own_len=lens,
+                   q_len=torch.randint(0, M + 1, (R,), generator=g).tolist() if i % 4 == 0 else None,
+                   causal=i % 5 < 2, seed=i))
+
+
 def test_equals_attention_over_the_joined_keys():
     """The same softmax as kernels.attention over prefix and own keys in a row."""
     from gpa_vggt_b200 import kernels

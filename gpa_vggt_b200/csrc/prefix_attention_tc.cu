@@ -121,6 +121,19 @@ struct Piece {
   int slot;          // which partial output
   bool first, last;  // holds the item's first, last step
 };
+// A piece from shared memory, read anew at each call: what the softmax needs after
+// its key tiles does not stay in registers meanwhile (a few more of them made its
+// loop 15% slower).
+__device__ __forceinline__ Piece read_piece(const Piece* at) {
+  const volatile Piece* v = at;
+  Piece c;
+  c.req = v->req; c.kh = v->kh; c.tile = v->tile;
+  c.len = v->len; c.qlen = v->qlen;
+  c.j0 = v->j0; c.nk = v->nk;
+  c.slot = v->slot;
+  c.first = v->first; c.last = v->last;
+  return c;
+}
 struct Walk {
   int pos, end, span;   // this CTA's units (all of a call's fit 31 bits)
   int req;
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   auto next = [&](Piece& c, uint32_t turn, bool& okw) {
     okw = wait(&piece_full[turn % RING], turn / RING);
     if (!okw) return false;
-    c = ring[turn % RING];
+    c = read_piece(&ring[turn % RING]);
     return c.req >= 0;
   };
   auto done = [&](uint32_t turn) {
@@ -548,13 +561,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     constexpr float kNoMax = -3.0e38f;   // no key yet
     int cs = 0, g = 0, ih = 0;   // ih: pieces in halves so far
     bool okw = true;
-    auto run = [&](const Piece& c) {
-      const int n = tiles_of(c, t, g);
-      const bool halves = HALVES && c.nk > 0, other = halves && tiles_of(c, 1, g) > 0;
-      const Row row = tile_row(p, tc, c.kh, c.req, c.tile + (HALVES ? 0 : t), row_i);
-      const bool idle = !__any_sync(0xffffffffu, row.live);   // a warp without rows only keeps the barriers going
-      // own keys that this row sees end here
-      const int limit = CAUSAL ? c.len - c.qlen + row.m + 1 : 0;
+    auto run = [&](const Piece& c0, const Piece* at) {
+      const int n = tiles_of(c0, t, g);
+      bool live;
+      int limit;   // own keys that this row sees end here
+      {
+        const Row row = tile_row(p, tc, c0.kh, c0.req, c0.tile + (HALVES ? 0 : t), row_i);
+        live = row.live;
+        limit = CAUSAL ? c0.len - c0.qlen + row.m + 1 : 0;
+      }
+      const bool idle = !__any_sync(0xffffffffu, live);   // a warp without rows only keeps the barriers going
       float m_raw = kNoMax, l = 0.f;       // running maximum (score units), row sum
       float neg_mc = 0.f;                  // -c2 * m_raw
       auto quarter = [&](float* xq, float neg, float* acc, uint32_t* pk) {
@@ -594,7 +610,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (D == 64 && lane == 0) bar_arrive(&s_empty[t]);
         if (CAUSAL) {   // keys ahead of this row
-          const Tile kt = tile_of(c, key_tile(t, j, g));
+          const Tile kt = tile_of(read_piece(at), key_tile(t, j, g));
           if (kt.own && __any_sync(0xffffffffu, limit < kt.key0 + TM)) {
             const int end = limit - kt.key0;
 #pragma unroll
@@ -611,7 +627,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         const float mt = max3_nan(max3_nan(mx[0], mx[0], mx[1]), mx[2], mx[3]);
         float alpha = 1.f;
         // the maximum moves: also the first time, and for a NaN (never for a row without keys)
-        const bool moved = row.live && !((mt - m_raw) * c2 <= 8.0f);
+        const bool moved = live && !((mt - m_raw) * c2 <= 8.0f);
         const bool any_moved = __any_sync(0xffffffffu, moved);
         if (any_moved) {
           if (moved) {
@@ -657,6 +673,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(&p_full[t]);
       }
+      const Piece c = read_piece(at);
+      const bool halves = HALVES && c.nk > 0, other = halves && tiles_of(c, 1, g) > 0;
       cs += n;
       g += c.nk;
       if (okw && n > 0) okw = wait(&o_done[t], cs - 1);
@@ -691,6 +709,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const bool some = m_raw > kNoMax;   // else the sum holds the polynomial's 2^-126
       const float inv = some ? 1.0f / l : 0.f;
       const bool direct = c.first && c.last && p.s2 == 0;
+      const Row row = tile_row(p, tc, c.kh, c.req, c.tile + (HALVES ? 0 : t), row_i);
       // the row tile among the partial outputs, and in this piece's slot
       const int block = (c.req * p.kv_heads + c.kh) * tc.tiles + c.tile + (HALVES ? 0 : t);
       const int64_t to = (int64_t)c.slot * tc.blocks + block;
@@ -748,7 +767,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     };
     Piece c;
     for (uint32_t turn = 0; okw && next(c, turn, okw); ++turn) {
-      run(c);
+      run(c, &ring[turn % RING]);
       done(turn);
     }
   }

@@ -586,9 +586,9 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   // Which kernels: the least time by a model in units of half a microsecond of an
   // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
   // 1.2 or 1.6 for 16, 32 or 64 rows (16 heads, 66,845 keys: 57, 74 and 94 us;
-  // mma.sync ends at 0.2-0.25 PFLOP/s); tc_kernel takes kPair or kSingle per step,
-  // or in halves, which wait for HBM, 3.5 (75 us for 64 rows), and 20 to start
-  // and end on every SM.
+  // mma.sync ends at 0.2-0.25 PFLOP/s).  A step of tc_kernel takes kPair or kSingle,
+  // in halves 5.5 (86 us for 64 rows, 89 for 128, where rows_kernel takes 187), and
+  // starting and ending take 20 on every SM, another launch for the caches 10.
   auto rows_cost = [&](int64_t rows, int64_t tiles) {
     const int wm = warps_for(rows);
     return (double)((rows + 16 * wm - 1) / (16 * wm)) * tiles * (wm == 1 ? 0.9 : wm == 2 ? 1.2 : 1.6) * kv_heads;
@@ -601,7 +601,8 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   for (int way = 0; way < 2; ++way) {   // joint, folded
     if (!(way ? fold && prefix > 0 : joint && prefix + (int64_t)cache > 0)) continue;
     if (!plan_tc(&tc, way, requests, queries, group, kv_heads, k1, k2, &total)) continue;
-    const double cost = (tc.halves ? total * 3.5 / kSingle : (double)total) + (way ? own_cost : 0) + 20.0 * kSms;
+    const double cost = (tc.halves ? total * 5.5 / kSingle : (double)total) + 20.0 * kSms +
+                        (way && cache > 0 ? own_cost + 10.0 * kSms : 0.0);
     if (cost < least) {
       least = cost;
       p.tc = tc;

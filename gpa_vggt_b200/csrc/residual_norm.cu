@@ -107,41 +107,51 @@ struct FwdParams {
   float* stats;        // [rows, 4]: mean, 1/std of y; mean, 1/std of z (or null)
 };
 
-// Sum over the WPR warps that share a row.  Every warp of the row's group calls
-// it the same number of times; two buffers in turn make one barrier enough.
+// Sums over the WPR warps that share a row, two at a time.  Every warp of the
+// row's group calls it the same number of times; two buffers in turn make one
+// barrier enough.
 template <int WPR>
 struct RowSum {
-  float* buf;   // [2][WPR] of this group
+  float2* buf;   // [2][WPR] of this group
   int bar, turn;
-  __device__ __forceinline__ float operator()(float s) {
+  __device__ __forceinline__ float2 operator()(float a, float b) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
     if constexpr (WPR > 1) {
-      float* b = buf + turn * WPR;
+      float2* w = buf + turn * WPR;
       turn ^= 1;
       const int warp = (threadIdx.x >> 5) % WPR;
-      if ((threadIdx.x & 31) == 0) b[warp] = s;
+      if ((threadIdx.x & 31) == 0) w[warp] = make_float2(a, b);
       asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(WPR * 32) : "memory");
-      s = 0.f;
+      a = b = 0.f;
 #pragma unroll
-      for (int i = 0; i < WPR; ++i) s += b[i];
+      for (int i = 0; i < WPR; ++i) {
+        a += w[i].x;
+        b += w[i].y;
+      }
     }
-    return s;
+    return make_float2(a, b);
   }
+  __device__ __forceinline__ float operator()(float a) { return (*this)(a, 0.f).x; }
 };
 
 // Forward.  WPR warps per row, VPL vectors of 8 columns per lane; a lane's
-// vectors past the row's end stay zero and are never loaded or stored.  One warp
-// per row up to 2,048 columns: all loads of a row are in flight at once and the
-// two sums of a norm are shuffles.  Eight warps per row above, so that a row
-// still fits the registers.
+// vectors past the row's end stay zero and are never loaded or stored.  A bf16
+// stream without a norm of the branch takes one warp per row up to 2,048 columns:
+// the sums are shuffles in layernorm's order, and 274,800 x 1,024 takes 372 us
+// (94% of the measured copy rate).  Elsewhere a lane takes at most four vectors,
+// two of fp32: 110,000 x 1,024 with an fp32 stream and a normed bf16 branch takes
+// 249 us (251 with two, 311 with one), with an fp32 branch 300 (365 with four).
 template <int VPL, int WPR, typename TX, typename TY>
 __global__ void __launch_bounds__(256) fwd_kernel(const FwdParams p) {
-  __shared__ float red[2 * 8];
-  const int t = threadIdx.x % (WPR * 32);
-  const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + threadIdx.x / (WPR * 32);
+  __shared__ float2 red[8 / WPR][2 * WPR];
+  const int t = threadIdx.x % (WPR * 32), grp = threadIdx.x / (WPR * 32);
+  const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + grp;
   if (row >= p.rows) return;   // whole groups leave together
-  RowSum<WPR> sum{red, 1, 0};
+  RowSum<WPR> sum{red[grp], 1 + grp, 0};
   const TX* xr = reinterpret_cast<const TX*>(p.x) + row * p.xs;
   const TY* yr = reinterpret_cast<const TY*>(p.y) + row * p.ys;
   const float n = (float)p.cols;
@@ -285,7 +295,8 @@ struct BwdParams {
 template <bool POST, int WPR, int VPT, typename TX, typename TY>
 __global__ void __launch_bounds__(WPR * 32 < 128 ? 128 : WPR * 32) bwd_kernel(const BwdParams p) {
   constexpr int NG = WPR * 32 < 128 ? 128 / (WPR * 32) : 1;
-  __shared__ float red[NG][4 * WPR];
+  asm volatile("griddepcontrol.launch_dependents;");   // the column sums may be launched, and wait for this grid's end
+  __shared__ float2 red[NG][2 * WPR];
   const int grp = threadIdx.x / (WPR * 32);
   const int t = threadIdx.x % (WPR * 32);
   const int worker = blockIdx.x * NG + grp;
@@ -371,8 +382,9 @@ __global__ void __launch_bounds__(WPR * 32 < 128 ? 128 : WPR * 32) bwd_kernel(co
     const bool more = p.whole ? next_g < p.groups : next < end;
     if (more) load_row(next);
     if (p.dh) {
-      s1 = p.kind == kLayer ? sum(s1) * inv_n : 0.f;
-      s2 = sum(s2) * inv_n;
+      const float2 s = sum(s1, s2);
+      s1 = p.kind == kLayer ? s.x * inv_n : 0.f;
+      s2 = s.y * inv_n;
     }
     float t1 = 0.f, t2 = 0.f;
     const int64_t grow = p.gate ? (int64_t)g * p.cols : 0;
@@ -412,8 +424,9 @@ __global__ void __launch_bounds__(WPR * 32 < 128 ? 128 : WPR * 32) bwd_kernel(co
       }
     }
     if constexpr (POST) {
-      t1 = p.post_kind == kLayer ? sum(t1) * inv_n : 0.f;
-      t2 = sum(t2) * inv_n;
+      const float2 s = sum(t1, t2);
+      t1 = p.post_kind == kLayer ? s.x * inv_n : 0.f;
+      t2 = s.y * inv_n;
 #pragma unroll
       for (int u = 0; u < VPT; ++u) {
         const int c = (u * WPR * 32 + t) * 8;
@@ -464,6 +477,7 @@ struct SumParams {
 // blockIdx.y: 0-3 the norm parameters, 4.. the gate groups.
 __global__ void __launch_bounds__(1024) sum_kernel(const SumParams p) {
   __shared__ float red[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // launched before the backward kernel's end
   const int cx = threadIdx.x & 31, wy = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
   const int slot = blockIdx.y < 4 ? (int)blockIdx.y + 1 : kGate;
@@ -533,10 +547,15 @@ template <typename TX, typename TY>
 static int launch_fwd(const FwdParams& p, cudaStream_t st) {
   const int vec = p.cols / 8;
 #define GPA_RN(V, W) fwd_kernel<V, W, TX, TY><<<(unsigned)((p.rows + 8 / W - 1) / (8 / W)), 256, 0, st>>>(p)
+  // few vectors per lane where a vector is many registers (fp32) or waits for many sums
+  const bool order = sizeof(TX) == 2 && p.post_kind == kNone, wide = sizeof(TY) == 4;
   if (vec <= 32) GPA_RN(1, 1);
   else if (vec <= 64) GPA_RN(2, 1);
-  else if (vec <= 128) GPA_RN(4, 1);
-  else if (vec <= 256) GPA_RN(8, 1);
+  else if (vec <= 128 && !wide) GPA_RN(4, 1);
+  else if (vec <= 128) GPA_RN(2, 2);
+  else if (vec <= 256 && order) GPA_RN(8, 1);
+  else if (vec <= 256 && !wide) GPA_RN(4, 2);
+  else if (vec <= 256) GPA_RN(2, 4);
   else if (vec <= 512) GPA_RN(2, 8);
   else GPA_RN(4, 8);
 #undef GPA_RN
@@ -654,6 +673,16 @@ extern "C" int gpa_residual_norm_backward(
   if (!gate_here && !dweight && !dbias && !dpost_weight && !dpost_bias) return ok();
   SumParams q{(const float*)workspace, cols, s.workers, s.per_group, gate_here ? groups : 0,
               {gate_here, dweight, dbias, dpost_weight, dpost_bias}, {gbf, pbf, pbf, pbf, pbf}};
-  sum_kernel<<<dim3((cols + 31) / 32, 4 + q.gate_groups), 1024, 0, st>>>(q);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((cols + 31) / 32, 4 + q.gate_groups);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sum_kernel, q);
+  if (e != cudaSuccess) return fail(GPA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }

@@ -58,8 +58,8 @@ struct TcSmem {
   static constexpr int V = K + STAGES * TILE;
   static constexpr int ONES = V + STAGES * TILE;
   static constexpr int BETA = ONES + XTILE;
-  static constexpr int MASK = BETA + STAGES * XTILE;   // 4 words per stage
-  static constexpr int ML = MASK + STAGES * 16;        // the second stream's maxima and sums
+  static constexpr int MASK = BETA + STAGES * XTILE;   // 4 words per key tile, twice as many as stages: V is used
+  static constexpr int ML = MASK + 2 * STAGES * 16;    // after its K's stage has gone on; the second stream's maxima and sums
   static constexpr int BARS = ML + TM * 8;
   static constexpr int TOTAL = BARS + 384;
   static constexpr int ALLOC = TOTAL + 1024;
@@ -120,6 +120,7 @@ struct Piece {
   int j0, nk;        // key tiles (nk may be 0: nothing to see here)
   int slot;          // which partial output
   bool first, last;  // holds the item's first, last step
+  bool single;       // the second row tile has no rows
 };
 // A piece from shared memory, read anew at each call: what the softmax needs after
 // its key tiles does not stay in registers meanwhile (a few more of them made its
@@ -132,6 +133,7 @@ __device__ __forceinline__ Piece read_piece(const Piece* at) {
   c.j0 = v->j0; c.nk = v->nk;
   c.slot = v->slot;
   c.first = v->first; c.last = v->last;
+  c.single = v->single;
   return c;
 }
 struct Walk {
@@ -162,6 +164,7 @@ __device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Wa
     b = (at + units + each - 1) / each;
     c.slot = blockIdx.x - (w.pos - at) / w.span;
     c.tile = pair * 2;
+    c.single = each == kSingle;
     w.pos += units;
   } while (a == b);   // the rest of a step that the CTA before has done
   c.req = w.req;
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           const Tile t = tile_of(c, j);
           if (!(okw = wait(&k_empty[s], ph + 1))) break;
           if (has_beta(t)) {
-            uint32_t* mask = reinterpret_cast<uint32_t*>(smem + SM::MASK + s * 16);
+            uint32_t* mask = reinterpret_cast<uint32_t*>(smem + SM::MASK + gk % (2 * ST) * 16);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const int row = u * 32 + lane;
@@ -429,97 +432,132 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const uint64_t dOnes = sdesc_plain(smem_u32(smem + SM::ONES));
       const uint64_t dBeta = sdesc_plain(smem_u32(smem + SM::BETA));
       const uint32_t dS = tbase + col_s(t), dO = tbase + col_o(t), dP = tbase + col_p(t);
+      // What follows a softmax's signal is kept short: the next tile's K, its bias
+      // and its rows to zero are seen to before.
       int i = 0, g = 0, cs = 0;   // cs: this stream's key tiles in earlier pieces
+      constexpr int STEP = HALVES ? 2 : 1;
+      int kst = HALVES ? t : 0, vst = kst;   // this stream's next K and V stage, and their phases
+      uint32_t kph = 0, vph = 0;
       bool okw = true;
+      // Zeroes the rows of key tile gt (of all pieces) that are out.  Where both
+      // issuers read a tile, the second writes the same zeros.
+      auto zero_rows = [&](int gt, uint8_t* tile) {
+        const uint4 m = *reinterpret_cast<const uint4*>(smem + SM::MASK + gt % (2 * ST) * 16);
+        if (!(m.x | m.y | m.z | m.w)) return;
+        tile += (lane >> 3) * SM::ATOM + (lane & 7) * 16;
+        for (int row = 0; row < TM; ++row) {
+          const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
+          if ((word >> (row & 31) & 1) && lane < 8 * SM::ATOMS)
+            *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_async_smem();
+        __syncwarp();
+      };
       auto run = [&](const Piece& c) {
         const int n = tiles_of(c, t, g);
         const uint64_t dQ = dQ0 + (uint64_t)((HALVES ? 0 : t) * (SM::TILE >> 4));
-        auto issue_s = [&](int j) {
-          const int jt = key_tile(t, j, g), st = (g + jt) % ST;
-          const bool beta = has_beta(tile_of(c, jt));
+        bool beta = false;
+        auto k_landed = [&](int j) {
+          const int jt = key_tile(t, j, g);
+          const Tile kt = tile_of(c, jt);
+          beta = has_beta(kt);
+          if (!wait(&k_full[kst], kph)) return false;
+          if (kt.own ? kt.valid < TM : p.bias != nullptr) zero_rows(g + jt, smem + SM::K + kst * SM::TILE);
+          return true;
+        };
+        auto v_landed = [&](int j) {
+          const int jt = key_tile(t, j, g);
+          const Tile kt = tile_of(c, jt);
+          if (!wait(&v_full[vst], vph)) return false;
+          if (kt.own ? kt.valid < TM : p.bias != nullptr) zero_rows(g + jt, smem + SM::V + vst * SM::TILE);
+          return true;
+        };
+        auto issue_s = [&](bool last) {
+          tc_fence_after();
           if (leader) {
-            const uint64_t bk = dK + (uint64_t)(st * (SM::TILE >> 4));
+            const uint64_t bk = dK + (uint64_t)(kst * (SM::TILE >> 4));
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t off = (uint64_t)((k >> 2) * (SM::ATOM >> 4) + (k & 3) * 2);
               umma_bf16(dS, dQ + off, bk + off, idesc_s, k != 0);
             }
-            if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(st * (XTILE >> 4)), idesc_s, 1);
+            if (beta) umma_bf16(dS, dOnes, dBeta + (uint64_t)(kst * (XTILE >> 4)), idesc_s, 1);
             umma_commit(&s_full[t]);
-            umma_commit(&k_empty[st]);
-            if (j == n - 1) umma_commit(q_empty);
+            umma_commit(&k_empty[kst]);
+            if (last) umma_commit(q_empty);
           }
           __syncwarp();
+          kst += STEP;
+          if (kst >= ST) {
+            kst -= ST;
+            kph ^= 1;
+          }
         };
-        auto issue_o = [&](int j) {
-          const int st = (g + key_tile(t, j, g)) % ST;
+        auto issue_o = [&](bool first) {
+          tc_fence_after();
           if (leader) {
-            const uint64_t bv = dV + (uint64_t)(st * (SM::TILE >> 4));
+            const uint64_t bv = dV + (uint64_t)(vst * (SM::TILE >> 4));
 #pragma unroll
             for (int ks = 0; ks < TM / 16; ++ks)
-              umma_bf16_ts(dO, dP + ks * 8, bv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0));
+              umma_bf16_ts(dO, dP + ks * 8, bv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (!first || ks > 0));
             umma_commit(&o_done[t]);
-            umma_commit(&v_empty[st]);
+            umma_commit(&v_empty[vst]);
           }
           __syncwarp();
-        };
-        // The rows to zero of a key tile, read once its K has landed (the producer
-        // reuses the words before its V is used).
-        auto rows_out = [&](int j) {
-          const int jt = key_tile(t, j, g);
-          const Tile kt = tile_of(c, jt);
-          return (kt.own ? kt.valid < TM : p.bias != nullptr)
-                     ? *reinterpret_cast<const uint4*>(smem + SM::MASK + ((g + jt) % ST) * 16)
-                     : make_uint4(0u, 0u, 0u, 0u);
-        };
-        // Where both issuers read a tile, the second writes the same zeros.
-        auto zero_rows = [&](const uint4& m, int base, int j) {
-          if (!(m.x | m.y | m.z | m.w)) return;
-          uint8_t* tile =
-              smem + base + ((g + key_tile(t, j, g)) % ST) * SM::TILE + (lane >> 3) * SM::ATOM + (lane & 7) * 16;
-          for (int row = 0; row < TM; ++row) {
-            const uint32_t word = row < 64 ? (row < 32 ? m.x : m.y) : (row < 96 ? m.z : m.w);
-            if ((word >> (row & 31) & 1) && lane < 8 * SM::ATOMS)
-              *reinterpret_cast<uint4*>(tile + row * 128) = make_uint4(0u, 0u, 0u, 0u);
+          vst += STEP;
+          if (vst >= ST) {
+            vst -= ST;
+            vph ^= 1;
           }
-          fence_async_smem();
-          __syncwarp();
-        };
-        auto wait_tile = [&](uint64_t* bar, int j) {
-          const int gt = g + key_tile(t, j, g);
-          return wait(&bar[gt % ST], gt / ST);
-        };
-        uint4 out_now = make_uint4(0u, 0u, 0u, 0u), out_next = out_now;
-        auto scores = [&](int j) {   // once K has landed and S is free
-          tc_fence_after();
-          out_next = rows_out(j);
-          zero_rows(out_next, SM::K, j);
-          issue_s(j);
         };
         okw = wait(q_full, i);
         if (okw && n == 0 && leader) bar_arrive(q_empty);   // nothing to read for this stream
+        if (!HALVES && t == 1 && c.single) {   // no rows: only the barriers go on
+          for (int j = 0; okw && j < n; ++j) {
+            okw = wait(&k_full[kst], kph);
+            if (!okw) break;
+            if (leader) {
+              bar_arrive(&s_full[t]);
+              bar_arrive(&k_empty[kst]);
+              if (j == n - 1) bar_arrive(q_empty);
+            }
+            kst = kst + 1 == ST ? 0 : kst + 1;
+            kph ^= kst == 0;
+            okw = wait(&p_full[t], cs + j) && wait(&v_full[vst], vph);
+            if (!okw) break;
+            if (leader) {
+              bar_arrive(&o_done[t]);
+              bar_arrive(&v_empty[vst]);
+            }
+            vst = vst + 1 == ST ? 0 : vst + 1;
+            vph ^= vst == 0;
+          }
+          cs += n;
+          return;
+        }
         if (okw && n > 0) {
           // S is free once the last softmax has read it, or (P in its place) the last product with V is done
-          okw = wait_tile(k_full, 0) && (cs == 0 || wait(D == 64 ? &s_empty[t] : &o_done[t], cs - 1));
-          if (okw) scores(0);
+          okw = k_landed(0) && (cs == 0 || wait(D == 64 ? &s_empty[t] : &o_done[t], cs - 1));
+          if (okw) issue_s(n == 1);
         }
         for (int j = 0; okw && j < n; ++j) {
-          out_now = out_next;
-          if (D == 64 && j + 1 < n) {
-            okw = wait(&s_empty[t], cs + j) && wait_tile(k_full, j + 1);
-            if (!okw) break;
-            scores(j + 1);
-          }
-          okw = wait(&p_full[t], cs + j) && wait_tile(v_full, j);
+          const bool more = j + 1 < n;
+          okw = v_landed(j) && (!more || k_landed(j + 1));
           if (!okw) break;
-          tc_fence_after();
-          zero_rows(out_now, SM::V, j);
-          issue_o(j);
-          if (D == 128 && j + 1 < n) {
-            // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
-            okw = wait_tile(k_full, j + 1) && wait(&o_done[t], cs + j);
-            if (!okw) break;
-            scores(j + 1);
+          if (D == 64) {
+            if (more) {
+              if (!(okw = wait(&s_empty[t], cs + j))) break;
+              issue_s(j + 2 == n);
+            }
+            if (!(okw = wait(&p_full[t], cs + j))) break;
+            issue_o(j == 0);
+          } else {
+            if (!(okw = wait(&p_full[t], cs + j))) break;
+            issue_o(j == 0);
+            if (more) {   // S(j+1) overwrites P(j), which O += P(j) V still reads until it is done
+              if (!(okw = wait(&o_done[t], cs + j))) break;
+              issue_s(j + 2 == n);
+            }
           }
         }
         cs += n;

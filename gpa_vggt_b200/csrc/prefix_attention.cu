@@ -563,9 +563,9 @@ static bool plan_tc(TcPlan* tc, bool fold, int requests, int queries, int group,
   const int64_t keys = std::max<int64_t>(prefix_tiles + (fold ? 0 : cache_tiles), 1);
   const int64_t steps = tc->halves ? (keys + 1) / 2 : keys;
   const int each = tiles > 1 ? kPair : kSingle;
-  const int64_t units = steps * each, least = std::min<int64_t>(kLeastSteps, steps) * each;
-  if ((double)(tiles / 2 * kPair + tiles % 2 * kSingle) * steps * heads >= 1e9 || (double)tiles * heads >= 1e7) return false;
-  *total = (tiles / 2 * kPair + tiles % 2 * kSingle) * steps * heads;
+  const int64_t units = (steps + kItemSteps) * each, least = std::min<int64_t>(kLeastSteps, steps) * each;
+  if ((double)(tiles + 1) * kPair * (steps + kItemSteps) * heads >= 1e9 || (double)tiles * heads >= 1e7) return false;
+  *total = (tiles / 2 * kPair + tiles % 2 * kSingle) * (steps + kItemSteps) * heads;
   const int64_t span = std::max((*total + kSms - 1) / kSms, least);
   const int64_t cuts = std::min(2 * ((units + span - 1) / span), std::max<int64_t>(units / least, 1));
   tc->blocks = (int)(tiles * heads);
@@ -586,7 +586,7 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   // Which kernels: the least time by a model in units of half a microsecond of an
   // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
   // 1.2 or 1.6 for 16, 32 or 64 rows (16 heads, 66,845 keys: 57, 74 and 94 us;
-  // mma.sync ends at 0.2-0.25 PFLOP/s).  A step of tc_kernel takes kPair or kSingle,
+  // mma.sync ends at 0.2-0.25 PFLOP/s).  A step of tc_kernel takes 3 or 2.4,
   // in halves 5.5 (86 us for 64 rows, 89 for 128, where rows_kernel takes 187), and
   // starting and ending take 20 on every SM, another launch for the caches 10.
   auto rows_cost = [&](int64_t rows, int64_t tiles) {
@@ -601,7 +601,7 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   for (int way = 0; way < 2; ++way) {   // joint, folded
     if (!(way ? fold && prefix > 0 : joint && prefix + (int64_t)cache > 0)) continue;
     if (!plan_tc(&tc, way, requests, queries, group, kv_heads, k1, k2, &total)) continue;
-    const double cost = (tc.halves ? total * 5.5 / kSingle : (double)total) + 20.0 * kSms +
+    const double cost = total * (tc.halves ? 5.5 / kSingle : 3.0 / kPair) + 20.0 * kSms +
                         (way && cache > 0 ? own_cost + 10.0 * kSms : 0.0);
     if (cost < least) {
       least = cost;

@@ -52,8 +52,10 @@ __device__ __forceinline__ int query_count(const Params& p, int r) {
 // What the sum of a row's first partial output holds when its output is written.
 constexpr float kWritten = -1.0f;
 
-// Units of time that a step of tc_kernel counts, with rows in two tiles or in one.
-constexpr int kPair = 3, kSingle = 2;
+// Units of time that a step of tc_kernel counts, with rows in two tiles (1.36 us at
+// head_dim 64, 2.4 at 128) or in one (1.11, 1.9), and the steps that beginning and
+// ending an item are worth.
+constexpr int kPair = 5, kSingle = 4, kItemSteps = 2;
 
 // The tensor-core kernel's share of a call: 128-row tiles over the prefix and,
 // unless `fold`, each request's own keys.

@@ -92,8 +92,8 @@ __device__ __forceinline__ void exp8(const float* x, float* e) {
 }
 
 // The order of work: requests, their key heads, the head's row-tile pairs, a
-// pair's steps (a key tile; two of them in halves).  A step of a pair with two
-// row tiles counts three units of time, of one two.
+// pair's steps (a key tile; two of them in halves) and kItemSteps more for its
+// ends.  A step of a pair with two row tiles counts kPair units, of one kSingle.
 struct Load {
   int pairs2;      // pairs with two row tiles
   bool single;     // and one with one
@@ -109,7 +109,7 @@ __device__ __forceinline__ Load load_of(const Params& p, const TcPlan& tc, int r
   w.single = tiles & 1;
   const int keys = max(1, (p.prefix + TM - 1) / TM + (tc.fold ? 0 : (own_length(p, r) + TM - 1) / TM));
   w.steps = HALVES ? (keys + 1) >> 1 : keys;
-  w.head = w.steps * (kPair * w.pairs2 + (w.single ? kSingle : 0));
+  w.head = (w.steps + kItemSteps) * (kPair * w.pairs2 + (w.single ? kSingle : 0));
   return w;
 }
 
@@ -155,18 +155,18 @@ __device__ __forceinline__ bool next_piece(const Params& p, const TcPlan& tc, Wa
     c.kh = x / ld.head;
     const int y = x - c.kh * ld.head;
     steps = ld.steps;
-    const int pair = min(y / (kPair * steps), ld.pairs2);
-    const int at = y - pair * (kPair * steps);   // units of the pair that others have
+    const int whole = kPair * (steps + kItemSteps), pair = min(y / whole, ld.pairs2);
+    const int at = y - pair * whole;   // units of the pair that others have
     const int each = pair < ld.pairs2 ? kPair : kSingle;
-    const int units = min(steps * each - at, w.end - w.pos);
+    const int units = min((steps + kItemSteps) * each - at, w.end - w.pos);
     // a step goes to the CTA that has its first unit
-    a = (at + each - 1) / each;
-    b = (at + units + each - 1) / each;
+    a = min(steps, (at + each - 1) / each);
+    b = min(steps, (at + units + each - 1) / each);
     c.slot = blockIdx.x - (w.pos - at) / w.span;
     c.tile = pair * 2;
     c.single = each == kSingle;
     w.pos += units;
-  } while (a == b);   // the rest of a step that the CTA before has done
+  } while (a == b);   // the rest of a step, or of an item, that the CTA before has done
   c.req = w.req;
   c.qlen = tc.fold ? p.queries : query_count(p, c.req);
   c.len = tc.fold ? 0 : own_length(p, c.req);

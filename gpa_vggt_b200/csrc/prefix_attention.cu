@@ -12,10 +12,14 @@
 // Scores, statistics and partial outputs are fp32; the probabilities are rounded
 // to bf16 for the product with V (their sum is not).
 //
-// Few rows per tile make this a stream of K and V from HBM: 16 to 64 rows on
-// mma.sync tiles, whose rate suffices there (64 rows need 64 flop per byte, 0.4
-// PFLOP/s at the full HBM rate).  K and V come through a cp.async ring of 64-key
-// tiles, three CTAs per SM (two at head_dim 128).
+// This file: few rows per tile (one token, or a few, of each request), 16 to 64
+// rows on mma.sync tiles.  Up to 16 rows a call is a stream of K and V from HBM: 5
+// streams of one token over 219,840 + 2,748 keys of 16 heads read 0.94 GB in 150 us
+// (97% of the measured copy rate).  From 32 rows on the tensor unit bounds it, which
+// ends at 0.2-0.25 PFLOP/s for mma.sync (64 rows over 66,845 keys: 83 us, 16 rows
+// 50).  K and V come through a cp.async ring of 64-key tiles, three CTAs per SM (two
+// at head_dim 128): 64 KB of loads in flight per CTA, and enough warps that one's
+// exponentials run beside another's products.  Many rows: prefix_attention_tc.cu.
 #include "prefix_attention.cuh"
 
 namespace gpa {

@@ -26,6 +26,13 @@
 // At head_dim 64 S, P and O of both streams fit TMEM side by side and S(j+1) runs
 // during the softmax of S(j).  At 128 P(j) takes the columns of S(j), and S(j+1)
 // waits for O += P(j) V; the other stream's softmax runs meanwhile.
+//
+// Bound by the softmax at head_dim 64 (issue slots and MUFU: 50% and 55% busy, the
+// tensor pipe 45%) and by the issuers' round trip at 128.  Whole tiles (9,472 rows
+// x 16,384 keys): 850 TFLOP/s for 16 heads of 64, 1,050-1,090 for 8 of 128.  Four
+// requests of 1,374 tokens over 16,711 + 1,374 keys: 542 us (one CTA per item 685:
+// 384 items end in a third of a wave).  In halves, 64 rows over 66,845 keys take 82
+// us, 128 rows 84, each stream waiting for its own chain of products and softmax.
 #include "prefix_attention.cuh"
 
 namespace gpa {

@@ -503,6 +503,9 @@ def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bi
     if lse_out is not None and (lse_out.dtype != F32 or lse_out.shape != (R, H, M)
                                 or (M > 1 and lse_out.stride(-1) != 1)):
         raise ValueError(f"{what}: lse_out must be an fp32 [R,H,M] view with row stride 1")
+    for t in (out, lse_out):
+        if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{what}: out and lse_out must not repeat rows (stride 0)")
     if torch.is_grad_enabled():
         for t in (q, k_prefix, v_prefix, k_own, v_own, bias):
             if t is not None and t.requires_grad:
@@ -533,7 +536,9 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
     -inf.  Nothing is read back to the host, so calls can be captured; no
-    gradients."""
+    gradients.  Many rows per key head run on the tensor cores, few as a stream of
+    the keys (the choice is by sizes and strides, not by values); a pipeline wait
+    that gives up is recorded in the device's status word (check_device_status)."""
     index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out)
     R, H, M, D = q.shape
     Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]

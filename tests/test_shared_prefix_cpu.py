@@ -34,6 +34,8 @@ def _args(R=2, H=4, M=3, D=64, Hk=2, P=5, N=7, dtype=BF16):
     (ValueError, {}, dict(out=torch.zeros(2, 4, 3, 64))),                 # not bf16
     (ValueError, {}, dict(out=torch.zeros(2, 4, 4, 64, dtype=BF16))),
     (ValueError, {}, dict(out=torch.zeros(2, 4, 3, 68, dtype=BF16)[..., :64])),   # rows not 16-byte aligned
+    (ValueError, {}, dict(out=torch.zeros(1, 4, 3, 64, dtype=BF16).expand(2, 4, 3, 64))),   # one row for two
+    (ValueError, {}, dict(lse_out=torch.zeros(2, 1, 3).expand(2, 4, 3))),
     (ValueError, {}, dict(lse_out=torch.zeros(2, 4, 3, dtype=BF16))),
     (ValueError, {}, dict(lse_out=torch.zeros(2, 3, 4).transpose(1, 2))),
     (ValueError, {}, {}),                                                 # all well, but on the CPU

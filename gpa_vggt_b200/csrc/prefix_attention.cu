@@ -549,9 +549,11 @@ struct Plan {
 static int warps_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 // The tensor-core kernel's share: over prefix and own keys of each request, or
-// folded over the prefix alone.  False where its counts would not fit.
+// folded over the prefix alone.  False where its counts would not fit, or a token's
+// query heads of one key head a 128-row tile.
 static bool plan_tc(TcPlan* tc, bool fold, int requests, int queries, int group, int kv_heads, int64_t prefix_tiles,
                     int64_t cache_tiles, int64_t* total) {
+  if (group > 128) return false;
   const int64_t tokens = fold ? (int64_t)requests * queries : queries;
   tc->fold = fold;
   tc->tokens = (int)tokens;

@@ -1,10 +1,14 @@
 """attention_shared_prefix refuses what it does not compute before anything is
 launched (no GPU needed: shapes and types are checked before the device)."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
 
+ROOT = pathlib.Path(__file__).resolve().parents[1]
 BF16, F32 = torch.bfloat16, torch.float32
 
 
@@ -92,3 +96,12 @@ def test_workspace_size(lib):
         row = (D + 2) * 4                                      # a partial output, its maximum and sum
         assert n % row == 0 and n >= R * M * H * row
         assert n < 1 << 28
+
+
+@pytest.mark.parametrize("heads", [128, 129, 256, 1000])
+def test_more_query_heads_than_a_tile_has_rows(lib, heads):
+    """One key head of more than 128 query heads: no whole token fits a 128-row tile."""
+    code = ("from gpa_vggt_b200 import _lib; "
+            f"print(_lib.load().gpa_attention_shared_prefix_workspace_bytes(2, 5, {heads}, 1, 64, 1000, 100))")
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert got.returncode == 0 and int(got.stdout.split()[-1]) >= 2 * 5 * heads * 66 * 4

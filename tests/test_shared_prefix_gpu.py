@@ -448,3 +448,8 @@ def test_public_form_casts_as_attention_keybias():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     with pytest.raises(NotImplementedError):
         attention_shared_prefix(*(f[k].half() for k in ("q", "k_prefix", "v_prefix", "k_own", "v_own")), None, 0.1)
+
+
+@pytest.mark.parametrize("size", [(2, 1, 129, 1, 64, 300, 40), (1, 3, 256, 1, 128, 130, 70), (2, 2, 400, 2, 64, 0, 65)])
+def test_more_query_heads_than_a_tile_has_rows(size):
+    check(make(*size, bias="key", own_len=[size[-1], 3][:size[0]], causal=True, seed=4))

@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(WPR * 32 < 128 ? 128 : WPR * 32) bwd_kernel(co
   };
   if (row < end) load_row(row);
   while (row < end) {
-    const float mean_y = st.x, rstd_y = st.y, mean = st.z, rstd = st.w;
+    const float mean_y = st.x, rstd_y = st.y;
+    const float mean = p.dh ? st.z : 0.f, rstd = p.dh ? st.w : 0.f;   // h unused: nothing comes through its norm, not even NaN
     float d[VPT][8], y8[VPT][8];
     float s1 = 0.f, s2 = 0.f;
     // N': the gradient through the norm of z

@@ -362,3 +362,17 @@ def test_block_calls_it_and_keeps_its_results(monkeypatch):
         y = layers._residual(x, block.ls1, block.attn(block.norm1(x)))
         ref = layers._residual(y, block.ls2, block.mlp(block.norm2(y)))
     assert calls == [1] and torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_unused_norm_of_a_row_that_is_not_finite(kind):
+    """With h unused, dx is dz for every row, as if there were no norm."""
+    from gpa_vggt_b200 import kernels
+    t = make((3, 5, 256), F32, BF16, BF16, "channel", kind, None)
+    x = t["x"].detach().clone()
+    x[1, 2, 7], x[2, 0, 9] = float("inf"), float("nan")
+    x.requires_grad_(True)
+    w = t["weight"].detach().clone().requires_grad_(True)
+    z, _ = kernels.residual_norm(x, t["y"], t["gate"], w, None, EPS, kind=kind)
+    dx, dw = torch.autograd.grad(z, [x, w], t["dz"])
+    assert torch.equal(dx, t["dz"]) and not bool(dw.any())

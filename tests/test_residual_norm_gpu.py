@@ -376,3 +376,32 @@ def test_unused_norm_of_a_row_that_is_not_finite(kind):
     z, _ = kernels.residual_norm(x, t["y"], t["gate"], w, None, EPS, kind=kind)
     dx, dw = torch.autograd.grad(z, [x, w], t["dz"])
     assert torch.equal(dx, t["dz"]) and not bool(dw.any())
+
+
+@pytest.mark.parametrize("how", ["hook", "pre_hook", "instance", "subclass"])
+def test_block_calls_a_norm_that_someone_watches(how):
+    """Hooks on norm2, and forwards put in its place, run as they would without the fused pass."""
+    from gpa_vggt_b200.vggt import layers
+    torch.manual_seed(1)
+    block = layers.Block(256, 4, init_values=0.3, qk_norm=True).cuda().bfloat16().eval()
+    x = torch.randn(2, 33, 256, device="cuda").bfloat16()
+    seen = []
+
+    class Watched(layers.LayerNorm):
+        def forward(self, x):
+            seen.append(x.shape)
+            return super().forward(x)
+
+    with torch.no_grad():
+        ref = block(x)
+        if how == "hook":
+            block.norm2.register_forward_hook(lambda m, i, o: seen.append(o.shape))
+        elif how == "pre_hook":
+            block.norm2.register_forward_pre_hook(lambda m, i: seen.append(i[0].shape))
+        elif how == "instance":
+            real = block.norm2.forward
+            block.norm2.forward = lambda x: seen.append(x.shape) or real(x)
+        else:
+            block.norm2.__class__ = Watched
+        out = block(x)
+    assert seen == [x.shape] and torch.equal(out, ref)

@@ -471,7 +471,32 @@ def _vectors(t: torch.Tensor):
     return t, t.stride()[:-1]
 
 
-def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out):
+def _span(t: torch.Tensor):
+    """(first, past the last) byte that t's elements lie in; empty tensors: nothing."""
+    if t.numel() == 0:
+        return 0, 0
+    n = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between a's ends meets that between b's."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _repeats(t: torch.Tensor) -> bool:
+    """Whether two indexes of t may be one place in memory: a stride within the
+    reach of the dims with smaller ones."""
+    reach = 0
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s <= reach:
+            return True
+        reach += (n - 1) * s
+    return False
+
+
+def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status):
     what = "attention_shared_prefix"
     if q.dim() != 4 or k_prefix.dim() != 3 or k_own.dim() != 4:
         raise ValueError(f"{what}: q [R,H,M,D], k_prefix [Hk,P,D] and k_own [R,Hk,N,D] required")
@@ -503,14 +528,23 @@ def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bi
     if lse_out is not None and (lse_out.dtype != F32 or lse_out.shape != (R, H, M)
                                 or (M > 1 and lse_out.stride(-1) != 1)):
         raise ValueError(f"{what}: lse_out must be an fp32 [R,H,M] view with row stride 1")
+    if P > 2 ** 30 or N > 2 ** 30 or R * M * H >= 2 ** 31:
+        raise ValueError(f"{what}: at most 2^30 prefix and own keys, fewer than 2^31 query rows")
     for t in (out, lse_out):
-        if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-            raise ValueError(f"{what}: out and lse_out must not repeat rows (stride 0)")
+        if t is None:
+            continue
+        if _repeats(t):
+            raise ValueError(f"{what}: out and lse_out must not repeat rows (overlapping strides)")
+        for u in (q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, None if t is lse_out else lse_out):
+            if u is not None and _meet(t, u):
+                raise ValueError(f"{what}: out and lse_out must lie outside the memory of the inputs and each other")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError(f"{what}: status must be one int32")
     if torch.is_grad_enabled():
         for t in (q, k_prefix, v_prefix, k_own, v_own, bias):
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
-    return _one_device(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, what=what)
+    return _one_device(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status, what=what)
 
 
 def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
@@ -535,11 +569,11 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     Returns out [R,H,M,D] bf16, and with return_lse (or lse_out) the log2 row
     sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
-    -inf.  Nothing is read back to the host, so calls can be captured; no
+    -inf.  `out` and `lse_out` lie outside the inputs' memory.  Nothing is read back to the host, so calls can be captured; no
     gradients.  Many rows per key head run on the tensor cores, few as a stream of
     the keys (the choice is by sizes and strides, not by values); a pipeline wait
     that gives up is recorded in the device's status word (check_device_status)."""
-    index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out)
+    index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status)
     R, H, M, D = q.shape
     Hk, P, N = k_prefix.shape[0], k_prefix.shape[1], k_own.shape[2]
     device = q.device

@@ -443,8 +443,9 @@ GPA_API int gpa_residual_norm_backward(
  * own_len may hold anything.  Query rows past q_len are neither computed nor
  * written.  causal: query i of a request sees its own keys j <= own_len - q_len
  * + i (the last query sees all); the prefix is seen by every query.  A query
- * without keys gives 0 and lse -inf.  lse: fp32, rows contiguous, or NULL.
- * workspace: 16-byte aligned, _workspace_bytes() (-1: bad sizes); calls that may
+ * without keys gives 0 and lse -inf.  lse: fp32, rows contiguous, or NULL.  o
+ * and lse overlap no input.  status: device int, set to 1 where a pipeline wait
+ * gives up, or NULL.  workspace: 16-byte aligned, _workspace_bytes() (-1: bad sizes); calls that may
  * overlap need their own.
  */
 GPA_API int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int queries, int heads, int kv_heads,

@@ -105,3 +105,43 @@ def test_more_query_heads_than_a_tile_has_rows(lib, heads):
             f"print(_lib.load().gpa_attention_shared_prefix_workspace_bytes(2, 5, {heads}, 1, 64, 1000, 100))")
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert got.returncode == 0 and int(got.stdout.split()[-1]) >= 2 * 5 * heads * 66 * 4
+
+
+def test_memory_that_is_written_is_not_read():
+    from gpa_vggt_b200 import kernels
+    args = _args()
+    with pytest.raises(ValueError, match="outside the memory"):
+        kernels.attention_shared_prefix(*args, out=args[0])
+    big = torch.zeros(8 + 2 * 2 * 7 * 64, dtype=BF16)           # out begins eight values ahead of k_own
+    args[3] = big[8:].view(2, 2, 7, 64)
+    with pytest.raises(ValueError, match="outside the memory"):
+        kernels.attention_shared_prefix(*args, out=big[:2 * 4 * 3 * 64].view(2, 4, 3, 64))
+    both = torch.zeros(2 * 4 * 3 * 64, dtype=BF16)
+    lse = both[:48].view(torch.float32).view(2, 4, 3)
+    with pytest.raises(ValueError, match="outside the memory"):
+        kernels.attention_shared_prefix(*_args(), out=both.view(2, 4, 3, 64), lse_out=lse)
+
+
+def test_outputs_whose_rows_overlap():
+    from gpa_vggt_b200 import kernels
+    buf = torch.zeros(4096, dtype=BF16)
+    with pytest.raises(ValueError, match="repeat rows"):
+        kernels.attention_shared_prefix(*_args(), out=buf.as_strided((2, 4, 3, 64), (64, 192, 64, 1)))
+    with pytest.raises(ValueError, match="CUDA device"):      # heads between the tokens: no overlap
+        kernels.attention_shared_prefix(*_args(), out=buf[:1536].view(2, 3, 4, 64).transpose(1, 2))
+
+
+@pytest.mark.parametrize("i", [1, 3])
+def test_more_keys_than_an_index_holds(i):
+    from gpa_vggt_b200 import kernels
+    args = _args(R=1, Hk=1)
+    for j in (i, i + 1):
+        args[j] = torch.zeros(1, dtype=BF16).expand(*args[j].shape[:-2], 2 ** 32 + 5, 64)
+    with pytest.raises(ValueError, match="2\\^30"):
+        kernels.attention_shared_prefix(*args)
+
+
+def test_status_word_of_another_type():
+    from gpa_vggt_b200 import kernels
+    with pytest.raises(ValueError, match="status"):
+        kernels.attention_shared_prefix(*_args(), status=torch.zeros(1))

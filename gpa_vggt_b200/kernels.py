@@ -538,8 +538,8 @@ def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bi
         for u in (q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, None if t is lse_out else lse_out):
             if u is not None and _meet(t, u):
                 raise ValueError(f"{what}: out and lse_out must lie outside the memory of the inputs and each other")
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
-        raise ValueError(f"{what}: status must be one int32")
+    if status is not None and (status.dtype != torch.int32 or status.numel() == 0):
+        raise ValueError(f"{what}: status must be int32")
     if torch.is_grad_enabled():
         for t in (q, k_prefix, v_prefix, k_own, v_own, bias):
             if t is not None and t.requires_grad:

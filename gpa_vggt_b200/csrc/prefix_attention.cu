@@ -16,10 +16,12 @@
 // rows on mma.sync tiles.  Up to 16 rows a call is a stream of K and V from HBM: 5
 // streams of one token over 219,840 + 2,748 keys of 16 heads read 0.94 GB in 150 us
 // (97% of the measured copy rate).  From 32 rows on the tensor unit bounds it, which
-// ends at 0.2-0.25 PFLOP/s for mma.sync (64 rows over 66,845 keys: 83 us, 16 rows
-// 50).  K and V come through a cp.async ring of 64-key tiles, three CTAs per SM (two
+// ends at 0.2-0.25 PFLOP/s for mma.sync (with the join, 16, 32 and 64 rows over
+// 66,845 keys of 16 heads: 58, 67 and 94 us).  K and V come through a cp.async ring of 64-key tiles, three CTAs per SM (two
 // at head_dim 128): 64 KB of loads in flight per CTA, and enough warps that one's
 // exponentials run beside another's products.  Many rows: prefix_attention_tc.cu.
+#include <type_traits>
+
 #include "prefix_attention.cuh"
 
 namespace gpa {
@@ -29,6 +31,7 @@ constexpr int BN = 64;         // keys per tile
 constexpr int THREADS = 128;
 constexpr int kSlotTiles = 2;  // at least this many tiles per chunk (2 requests, 2,361 + 100 keys: 8.3 us; 4: 8.9)
 constexpr int kSms = 148;
+constexpr int kJoinCtas = kSms * 8;   // the most CTAs of join_tiles_kernel with 8 features a thread
 constexpr int kLeastSteps = 4;  // the tensor-core kernel cuts no item into parts of fewer steps
 
 template <int D>
@@ -464,12 +467,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 }
 
 // Joins tc_kernel's parts (and rows_kernel's chunks of the caches, in a folded
-// call): a thread per row of a 128-row tile, 32 features of it.  Rows whose output
-// is written already leave at once.
-template <int D>
+// call): a thread per row of a 128-row tile, F features of it.  FEW tiles are cut
+// into many parts, and the time is the latency of their loads in turn: 8 features a
+// thread and 8 parts in flight hide it (128 rows over 66,845 keys: 77 us with
+// tc_kernel, 85 with 32 features and a part at a time; 7 requests of 45 tokens: 41
+// and 48).  Many tiles fill the GPU with 32 features, in longer runs of a row (3 x
+// 515 tokens: 107 us, 112 with 8; 8 x 300 over 8,191 + 1,030 keys: 191 and 204).
+// Rows whose output is written already leave at once.
+template <int D, bool FEW>
 __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const TcPlan tc) {
+  constexpr int F = FEW ? 8 : 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int i = threadIdx.x, block = blockIdx.x, f0 = blockIdx.y * 32;
+  const int i = threadIdx.x, block = blockIdx.x, f0 = blockIdx.y * F;
   const int rk = block / tc.tiles, req = rk / p.kv_heads, kh = rk - req * p.kv_heads;
   const Row w = tile_row(p, tc, kh, req, block - rk * tc.tiles, i);
   if (!w.live) return;
@@ -480,38 +489,66 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const T
   const int64_t row = row_index(p, w);
   const int slots = p.s1 + p.s2;
   float mx = first.x;
-#pragma unroll 4
+#pragma unroll FEW ? 8 : 4
   for (int s = 1; s < tc.slots; ++s) mx = fmaxf(mx, tml[s * tstep].x);
-#pragma unroll 4
+#pragma unroll FEW ? 8 : 4
   for (int s = 0; s < slots; ++s) mx = fmaxf(mx, p.ws_ml[s * p.rows + row].x);
-  float l = 0.f, v[32];
+  float l = 0.f, v[F];
 #pragma unroll
-  for (int u = 0; u < 32; ++u) v[u] = 0.f;
+  for (int u = 0; u < F; ++u) v[u] = 0.f;
   // one part: its weight, and where it wrote any output, that
-  auto add = [&](const float2 ml, const float4* o, int64_t step) {
+  auto weight = [&](const float2 ml) {
     const float f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
     l = fmaf(ml.y, f, l);
-    if (f > 0.f) {
-      float4 x[8];
+    return f;
+  };
+  auto add = [&](float f, const float4* x) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = o[u * step];
+    for (int u = 0; u < F / 4; ++u) {
+      v[4 * u] = fmaf(f, x[u].x, v[4 * u]);
+      v[4 * u + 1] = fmaf(f, x[u].y, v[4 * u + 1]);
+      v[4 * u + 2] = fmaf(f, x[u].z, v[4 * u + 2]);
+      v[4 * u + 3] = fmaf(f, x[u].w, v[4 * u + 3]);
+    }
+  };
+  auto join = [&](int n, const float2* ml, int64_t ml_step, const float4* o, int64_t o_step, auto f_step) {
+    if constexpr (FEW) {
+      constexpr int AHEAD = 8;
+      for (int s0 = 0; s0 < n; s0 += AHEAD) {
+        float f[AHEAD];
+        float4 x[AHEAD][F / 4];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        v[4 * u] = fmaf(f, x[u].x, v[4 * u]);
-        v[4 * u + 1] = fmaf(f, x[u].y, v[4 * u + 1]);
-        v[4 * u + 2] = fmaf(f, x[u].z, v[4 * u + 2]);
-        v[4 * u + 3] = fmaf(f, x[u].w, v[4 * u + 3]);
+        for (int a = 0; a < AHEAD; ++a) f[a] = weight(s0 + a < n ? ml[(s0 + a) * ml_step] : make_float2(-INFINITY, 0.f));
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+          for (int u = 0; u < F / 4; ++u)
+            x[a][u] = f[a] > 0.f ? o[(s0 + a) * o_step + u * f_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) add(f[a], x[a]);
+      }
+    } else {
+      constexpr int kUnroll = decltype(f_step)::value == 1 ? 4 : 1;   // a request's chunks are many, a tile's parts two or three
+#pragma unroll kUnroll
+      for (int s = 0; s < n; ++s) {
+        const float f = weight(ml[s * ml_step]);
+        if (f > 0.f) {
+          float4 x[F / 4];
+#pragma unroll
+          for (int u = 0; u < F / 4; ++u) x[u] = o[s * o_step + u * f_step];
+          add(f, x);
+        }
       }
     }
   };
-  for (int s = 0; s < tc.slots; ++s)
-    add(tml[s * tstep], p.tc_o + (((int64_t)s * tc.blocks + block) * (D / 4) + f0 / 4) * 128 + i, 128);
-  for (int s = 0; s < slots; ++s)
-    add(p.ws_ml[s * p.rows + row], reinterpret_cast<const float4*>(p.ws_o + (s * p.rows + row) * D + f0), 1);
+  join(tc.slots, tml, tstep, p.tc_o + ((int64_t)block * (D / 4) + f0 / 4) * 128 + i, (int64_t)tc.blocks * (D / 4) * 128,
+       std::integral_constant<int, 128>());
+  join(slots, p.ws_ml + row, p.rows, reinterpret_cast<const float4*>(p.ws_o + row * D + f0), p.rows * (D / 4),
+       std::integral_constant<int, 1>());
   const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
   uint4* dst = reinterpret_cast<uint4*>(p.o + w.r * p.o_sr + w.h * p.o_sh + w.m * p.o_sm + f0);
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
+  for (int u = 0; u < F / 8; ++u)
     dst[u] = make_uint4(pack_bf16x2(v[8 * u] * inv, v[8 * u + 1] * inv), pack_bf16x2(v[8 * u + 2] * inv, v[8 * u + 3] * inv),
                         pack_bf16x2(v[8 * u + 4] * inv, v[8 * u + 5] * inv), pack_bf16x2(v[8 * u + 6] * inv, v[8 * u + 7] * inv));
   if (p.lse && f0 == 0) p.lse[w.r * p.lse_sr + w.h * p.lse_sh + w.m] = l == 0.f ? -INFINITY : mx + log2f(l);
@@ -591,10 +628,10 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   p.rows = r1 * kv_heads;
   // Which kernels: the least time by a model in units of half a microsecond of an
   // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
-  // 1.2 or 1.6 for 16, 32 or 64 rows (16 heads, 66,845 keys: 57, 74 and 94 us;
-  // mma.sync ends at 0.2-0.25 PFLOP/s).  A step of tc_kernel takes 3 or 2.4,
-  // in halves 5.5 (86 us for 64 rows, 89 for 128, where rows_kernel takes 187), and
-  // starting and ending take 20 on every SM, another launch for the caches 10.
+  // 1.2 or 1.6 for 16, 32 or 64 rows.  A step of tc_kernel takes 3 or 2.4, in
+  // halves 5.5, and starting and ending take 20 on every SM, another launch for the
+  // caches 10.  Measured on both sides (16 heads, 66,845 keys, us): 32 rows 67 here;
+  // 48 rows 93 and 76 there, 64 rows 94 and 76, 128 rows 188 and 77.
   auto rows_cost = [&](int64_t rows, int64_t tiles) {
     const int wm = warps_for(rows);
     return (double)((rows + 16 * wm - 1) / (16 * wm)) * tiles * (wm == 1 ? 0.9 : wm == 2 ? 1.2 : 1.6) * kv_heads;
@@ -660,7 +697,9 @@ static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
     }
   }
   if (rc) return rc;
-  if (tc) return launch_early(join_tiles_kernel<D>, dim3(plan.tc.blocks, D / 32), 128, 0, st, p, plan.tc);
+  if (tc && (int64_t)plan.tc.blocks * (D / 8) <= kJoinCtas)
+    return launch_early(join_tiles_kernel<D, true>, dim3(plan.tc.blocks, D / 8), 128, 0, st, p, plan.tc);
+  if (tc) return launch_early(join_tiles_kernel<D, false>, dim3(plan.tc.blocks, D / 32), 128, 0, st, p, plan.tc);
   // eight warps per row where that is few rows' shorter way (32 rows of 20 chunks: 8.3 us with the kernel before, 11.3
   // with one)
   if (p.s1 + p.s2 > 4 && p.rows <= 16384)

@@ -628,23 +628,26 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   p.rows = r1 * kv_heads;
   // Which kernels: the least time by a model in units of half a microsecond of an
   // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
-  // 1.2 or 1.6 for 16, 32 or 64 rows.  A step of tc_kernel takes 3 or 2.4, in
-  // halves 5.5, and starting and ending take 20 on every SM, another launch for the
-  // caches 10.  Measured on both sides (16 heads, 66,845 keys, us): 32 rows 67 here;
-  // 48 rows 93 and 76 there, 64 rows 94 and 76, 128 rows 188 and 77.
+  // 1.2 or 1.6 for 16, 32 or 64 rows; caches on fewer rows than the prefix wait for
+  // HBM while its products run, and cost a third less beside it (64 requests over
+  // 66,845 + 1,374 keys: 138 us, where each alone takes 94 and 67).  A step of
+  // tc_kernel takes 3 or 2.4, in halves 4.5, and starting and ending take 20 on every
+  // SM, another launch for the caches 10.  Measured on both sides (16 heads, 66,845
+  // keys, us): 32 rows 67 here; 48 rows 93 and 76 there, 64 rows 94 and 76, 128 rows
+  // 188 and 77; 64 rows with caches of 300 113 and 98, of 1,374 138 and 144.
   auto rows_cost = [&](int64_t rows, int64_t tiles) {
     const int wm = warps_for(rows);
     return (double)((rows + 16 * wm - 1) / (16 * wm)) * tiles * (wm == 1 ? 0.9 : wm == 2 ? 1.2 : 1.6) * kv_heads;
   };
   const double own_cost = requests * rows_cost(r2, t2);
-  double least = rows_cost(r1, t1) + own_cost;
+  double least = rows_cost(r1, t1) + own_cost * (prefix > 0 && warps_for(r2) < warps_for(r1) ? 0.65 : 1.0);
   TcPlan tc{};
   int64_t total = 0;
   const int64_t k1 = (prefix + 127) / 128, k2 = (cache + 127) / 128;
   for (int way = 0; way < 2; ++way) {   // joint, folded
     if (!(way ? fold && prefix > 0 : joint && prefix + (int64_t)cache > 0)) continue;
     if (!plan_tc(&tc, way, requests, queries, group, kv_heads, k1, k2, &total)) continue;
-    const double cost = total * (tc.halves ? 5.5 / kSingle : 3.0 / kPair) + 20.0 * kSms +
+    const double cost = total * (tc.halves ? 4.5 / kSingle : 3.0 / kPair) + 20.0 * kSms +
                         (way && cache > 0 ? own_cost + 10.0 * kSms : 0.0);
     if (cost < least) {
       least = cost;

@@ -14,12 +14,13 @@
 //
 // This file: few rows per tile (one token, or a few, of each request), 16 to 64
 // rows on mma.sync tiles.  Up to 16 rows a call is a stream of K and V from HBM: 5
-// streams of one token over 219,840 + 2,748 keys of 16 heads read 0.94 GB in 150 us
-// (97% of the measured copy rate).  From 32 rows on the tensor unit bounds it, which
-// ends at 0.2-0.25 PFLOP/s for mma.sync (with the join, 16, 32 and 64 rows over
-// 66,845 keys of 16 heads: 58, 67 and 94 us).  K and V come through a cp.async ring of 64-key tiles, three CTAs per SM (two
-// at head_dim 128): 64 KB of loads in flight per CTA, and enough warps that one's
-// exponentials run beside another's products.  Many rows: prefix_attention_tc.cu.
+// streams of one token over 219,840 + 2,748 keys of 16 heads read 0.94 GB in 143 us
+// (6.57 TB/s).  From 32 rows on the tensor unit bounds it, which ends at 0.2-0.25
+// PFLOP/s for mma.sync (with the join, 16, 32 and 64 rows over 66,845 keys of 16
+// heads: 55, 62 and 95 us).  K and V come through a cp.async ring of three 64-key
+// tiles, with two to four CTAs per SM: 64 KB and more of loads in flight, and enough
+// warps that one's exponentials run beside another's products.  Many rows:
+// prefix_attention_tc.cu.
 #include <type_traits>
 
 #include "prefix_attention.cuh"
@@ -34,13 +35,21 @@ constexpr int kSms = 148;
 constexpr int kJoinCtas = kSms * 8;   // the most CTAs of join_tiles_kernel with 8 features a thread
 constexpr int kLeastSteps = 4;  // the tensor-core kernel cuts no item into parts of fewer steps
 
+// CTAs per SM for row tiles of 16 * wm1 rows over the prefix and 16 * wm2 over the
+// caches.  At head_dim 64 four with a ring of three tiles hide more of the loads and
+// of each other's exponentials than three with one of four (5 streams over 219,840 +
+// 2,748 keys 143 us, 147; 64 over 66,845 + 1,374 113, 116), but 32-row tiles, and
+// higher ones over the caches, need more than the 128 registers that leaves (32 rows
+// over 66,845 keys: 62 us with three, 66 with four; 8 x 64 tokens over 2,000 32, 34).
+constexpr int resident(int head_dim, int wm1, int wm2) { return head_dim == 128 ? 2 : wm2 == 1 && wm1 != 2 ? 4 : 3; }
+
 template <int D>
 struct Cfg {
-  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int STAGES = 3;
   static constexpr int TILE = BN * D * 2;                    // bytes of a K or V tile
   static constexpr int STAGE = 2 * TILE + BN * 4;            // K, V, bias
   static constexpr int SMEM = STAGES * STAGE;
-  static constexpr int CTAS = D == 64 ? 3 : 2;
+  static constexpr int CTAS = D == 64 ? 4 : 2;               // resident at most
   static_assert(SMEM * CTAS <= 227 * 1024 - CTAS * 1024, "shared memory of the resident CTAs");
   static_assert(4 * 16 * (D + 2) * 4 <= SMEM, "the warps' partial outputs reuse the ring");
 };
@@ -345,7 +354,7 @@ __device__ __forceinline__ void run_item(const Params& p, uint8_t* smem, int kh,
 }
 
 template <int D, int WM1, int WM2>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, resident(D, WM1, WM2)) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   asm volatile("griddepcontrol.launch_dependents;");   // the join may be launched, and waits for this grid's end
   // items of the prefix: row tile fastest (its CTAs share the keys in L2)
@@ -368,38 +377,40 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the chunks of a row with W warps (1: a warp's own row, 8: the block's).
+// Joins the chunks of a row with W warps (1: a warp's own row, else the block's,
+// which take the chunks in turn and are joined like chunks themselves).
 template <int D, int W>
-__device__ __forceinline__ void join_row(const Params& p, int64_t row, float (*part)[D]) {
+__device__ __forceinline__ void join_row(const Params& p, int64_t row, float (*part)[D], float2* part_ml) {
   constexpr int F = D / 32;   // features per lane
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int U = 8;        // loads in flight
+  const int warp = W == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = (int)((uint32_t)row % (uint32_t)p.heads), tok = (int)((uint32_t)row / (uint32_t)p.heads);
   const int m = (int)((uint32_t)tok % (uint32_t)p.queries), r = (int)((uint32_t)tok / (uint32_t)p.queries);
-  const int slots = p.s1 + p.s2;
-  const float2* mlr = p.ws_ml + row;
-  const float2 first = lane < slots ? mlr[lane * p.rows] : make_float2(-INFINITY, 0.f);
+  const int slots = (p.s1 + p.s2 - warp + W - 1) / W;   // this warp's: warp, warp + W, ...
+  const int64_t step = W * p.rows;
+  const float2* mlr = p.ws_ml + warp * p.rows + row;
+  const float2 first = lane < slots ? mlr[lane * step] : make_float2(-INFINITY, 0.f);
   float mx = first.x;
-  for (int s = lane + 32; s < slots; s += 32) mx = fmaxf(mx, mlr[s * p.rows].x);
+  for (int s = lane + 32; s < slots; s += 32) mx = fmaxf(mx, mlr[s * step].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float l = 0.f, v[F];
 #pragma unroll
   for (int u = 0; u < F; ++u) v[u] = 0.f;
-  const float* orow = p.ws_o + row * D + lane * F;
+  const float* orow = p.ws_o + (warp * p.rows + row) * D + lane * F;
   for (int s0 = 0; s0 < slots; s0 += 32) {
-    const float2 ml = s0 == 0 ? first : (s0 + lane < slots ? mlr[(s0 + lane) * p.rows] : make_float2(-INFINITY, 0.f));
+    const float2 ml = s0 == 0 ? first : (s0 + lane < slots ? mlr[(s0 + lane) * step] : make_float2(-INFINITY, 0.f));
     const float f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
     l = fmaf(ml.y, f, l);
     const int n = min(32, slots - s0);
-    constexpr int U = 8;   // loads in flight
-    for (int i0 = W == 1 ? 0 : warp; i0 < n; i0 += U * W) {
+    for (int i0 = 0; i0 < n; i0 += U) {
       float x[U][F], w[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const int s = i0 + i * W;
+        const int s = i0 + i;
         w[i] = __shfl_sync(0xffffffffu, f, s & 31);
         if (s >= n) w[i] = 0.f;
-        const float* src = orow + (int64_t)(s0 + s) * p.rows * D;
+        const float* src = orow + (s0 + s) * step * D;
         if (w[i] > 0.f) {   // an empty chunk wrote no output
           if constexpr (F == 2) {
             const float2 t = *reinterpret_cast<const float2*>(src);
@@ -424,13 +435,21 @@ __device__ __forceinline__ void join_row(const Params& p, int64_t row, float (*p
   if constexpr (W > 1) {
 #pragma unroll
     for (int u = 0; u < F; ++u) part[warp][lane * F + u] = v[u];
+    if (lane == 0) part_ml[warp] = make_float2(mx, l);
     __syncthreads();
     if (warp > 0) return;
 #pragma unroll
-    for (int u = 0; u < F; ++u) {
-      v[u] = 0.f;
+    for (int i = 0; i < W; ++i) mx = fmaxf(mx, part_ml[i].x);
+    l = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[u] += part[i][lane * F + u];
+    for (int u = 0; u < F; ++u) v[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float2 ml = part_ml[i];
+      const float f = ml.x > -INFINITY ? exp2f(ml.x - mx) : 0.f;
+      l = fmaf(ml.y, f, l);
+#pragma unroll
+      for (int u = 0; u < F; ++u) v[u] = fmaf(f, part[i][lane * F + u], v[u]);
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
@@ -451,18 +470,19 @@ __device__ __forceinline__ bool to_join(const Params& p, int64_t row) {
   return (int)(tok % (uint32_t)p.queries) < __ldg(p.q_len + tok / (uint32_t)p.queries);
 }
 
-// Joins rows_kernel's chunks.  WIDE: a block per row, each warp taking every
-// eighth chunk, else a warp per row.  The launch overlaps the end of the kernel
-// before it (a programmatic dependency), which the first line waits for.
-template <int D, bool WIDE>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+// Joins rows_kernel's chunks, a row with W warps (1, or a block of them).  The launch
+// overlaps the end of the kernel before it (a programmatic dependency), which the
+// first line waits for.
+template <int D, int W>
+__global__ void __launch_bounds__(W == 1 ? 256 : W * 32) join_kernel(const Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if constexpr (WIDE) {
-    __shared__ float part[8][D];
-    if (to_join(p, blockIdx.x)) join_row<D, 8>(p, blockIdx.x, part);
+  if constexpr (W > 1) {
+    __shared__ float part[W][D];
+    __shared__ float2 part_ml[W];
+    if (to_join(p, blockIdx.x)) join_row<D, W>(p, blockIdx.x, part, part_ml);
   } else {
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (to_join(p, row)) join_row<D, 1>(p, row, nullptr);
+    if (to_join(p, row)) join_row<D, 1>(p, row, nullptr, nullptr);
   }
 }
 
@@ -630,11 +650,11 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
   // SM at head_dim 64 (twice that at 128).  A 64-key tile of rows_kernel takes 0.9,
   // 1.2 or 1.6 for 16, 32 or 64 rows; caches on fewer rows than the prefix wait for
   // HBM while its products run, and cost a third less beside it (64 requests over
-  // 66,845 + 1,374 keys: 138 us, where each alone takes 94 and 67).  A step of
+  // 66,845 + 1,374 keys: 127 us, where each alone takes 95 and 64).  A step of
   // tc_kernel takes 3 or 2.4, in halves 4.5, and starting and ending take 20 on every
   // SM, another launch for the caches 10.  Measured on both sides (16 heads, 66,845
-  // keys, us): 32 rows 67 here; 48 rows 93 and 76 there, 64 rows 94 and 76, 128 rows
-  // 188 and 77; 64 rows with caches of 300 113 and 98, of 1,374 138 and 144.
+  // keys, us): 32 rows 62 here; 48 rows 93 and 76 there, 64 rows 95 and 76, 128 rows
+  // 166 and 77; 64 rows with caches of 300 100 and 95, of 1,374 127 and 144.
   auto rows_cost = [&](int64_t rows, int64_t tiles) {
     const int wm = warps_for(rows);
     return (double)((rows + 16 * wm - 1) / (16 * wm)) * tiles * (wm == 1 ? 0.9 : wm == 2 ? 1.2 : 1.6) * kv_heads;
@@ -665,7 +685,7 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
     const int64_t units = kv_heads * (p.rt1 * tiles1 + (int64_t)requests * p.rt2 * t2);
     // two items per resident CTA: short enough to even out requests of unequal
     // lengths, long enough that the partial outputs are a small share
-    const int64_t want = (int64_t)kSms * (head_dim == 64 ? 3 : 2) * 2;
+    const int64_t want = (int64_t)kSms * resident(head_dim, p.wm1, p.wm2) * 2;
     const int64_t per = std::max<int64_t>((units + want - 1) / want, kSlotTiles);
     p.chunk = (int)std::min<int64_t>(per, 1 << 24) * BN;
     p.s1 = (int)((tiles1 + per - 1) / per);
@@ -703,11 +723,21 @@ static int launch(const Params& p, const Plan& plan, cudaStream_t st) {
   if (tc && (int64_t)plan.tc.blocks * (D / 8) <= kJoinCtas)
     return launch_early(join_tiles_kernel<D, true>, dim3(plan.tc.blocks, D / 8), 128, 0, st, p, plan.tc);
   if (tc) return launch_early(join_tiles_kernel<D, false>, dim3(plan.tc.blocks, D / 32), 128, 0, st, p, plan.tc);
-  // eight warps per row where that is few rows' shorter way (32 rows of 20 chunks: 8.3 us with the kernel before, 11.3
-  // with one)
-  if (p.s1 + p.s2 > 4 && p.rows <= 16384)
-    return launch_early(join_kernel<D, true>, dim3((unsigned)p.rows), 256, 0, st, p);
-  return launch_early(join_kernel<D, false>, dim3((unsigned)((p.rows + 7) / 8)), 256, 0, st, p);
+  const int slots = p.s1 + p.s2;
+  auto join = [&](auto w) {
+    constexpr int W = decltype(w)::value;
+    return launch_early(join_kernel<D, W>, dim3((unsigned)p.rows), W * 32, 0, st, p);
+  };
+  // Warps per row: as many as its chunks feed, while the rows alone do not fill the
+  // GPU.  With the kernel before, us, at 32, 8, 4, 2 and 1 warps: one head over
+  // 200,000 keys (592 chunks) 25, 33; 16 rows of 16 heads over 66,845 (75) -, 55, 56,
+  // 59; 12 rows of 16 heads over 4,000 (11) -, 15.7, 14.0, 14.6, 20; 18 x 2 tokens of
+  // 64 heads (10) -, 22, 18.7, 16.5, 17.4; 8 x 64 tokens of 16 -, 56, 43, 36, 32.
+  if (slots > 128) return join(std::integral_constant<int, 32>());
+  if (slots > 32) return join(std::integral_constant<int, 8>());
+  if (slots > 4 && p.rows <= 1280) return join(std::integral_constant<int, 4>());
+  if (slots > 4 && p.rows <= 3000) return join(std::integral_constant<int, 2>());
+  return launch_early(join_kernel<D, 1>, dim3((unsigned)((p.rows + 7) / 8)), 256, 0, st, p);
 }
 
 static int check_sizes(const char* what, int requests, int queries, int heads, int kv_heads, int head_dim, int prefix,

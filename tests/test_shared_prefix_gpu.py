@@ -453,3 +453,16 @@ def test_public_form_casts_as_attention_keybias():
 @pytest.mark.parametrize("size", [(2, 1, 129, 1, 64, 300, 40), (1, 3, 256, 1, 128, 130, 70), (2, 2, 400, 2, 64, 0, 65)])
 def test_more_query_heads_than_a_tile_has_rows(size):
     check(make(*size, bias="key", own_len=[size[-1], 3][:size[0]], causal=True, seed=4))
+
+
+@pytest.mark.parametrize("size,own_len", [
+    ((1, 1, 1, 1, 64, 20000, 0), None),            # more than 128 chunks of a row
+    ((2, 1, 1, 1, 128, 20000, 90), [90, 0]),
+    ((2, 1, 4, 4, 64, 9000, 70), [0, 70]),         # more than 32
+    ((4, 12, 16, 4, 64, 0, 1500), [1500, 0, 3, 700]),   # four warps a row
+    ((18, 2, 32, 16, 64, 1288, 54), None),         # two
+    ((8, 64, 16, 16, 64, 0, 700), [700, 64, 0, 1, 699, 300, 65, 10]),   # one, of many rows
+    ((3, 40, 16, 2, 128, 2500, 200), [200, 0, 41]),     # few row tiles in many parts
+])
+def test_every_width_of_the_join(size, own_len):
+    check(make(*size, bias="key" if size[5] else None, own_len=own_len, causal=True, seed=6))

@@ -459,16 +459,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
 
 def _vectors(t: torch.Tensor):
     """(t or a copy of it, strides of all dims but the last, 0 where a dim has at
-    most one entry): innermost dim contiguous, 16-byte aligned vectors."""
-    if t.is_contiguous():
-        if aligned(t):
-            return t, t.stride()[:-1]
-    else:
+    most one entry: what stands there says nothing, also where t counts as
+    contiguous): innermost dim contiguous, 16-byte aligned vectors."""
+    if t.numel() == 0:
+        return t, (0,) * (t.dim() - 1)
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    if t.stride(-1) != 1 or not aligned(t) or any(s % 8 for s in strides[:-1]):
+        t = t.clone(memory_format=torch.contiguous_format)
         strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-        if t.stride(-1) == 1 and aligned(t) and not any(s % 8 for s in strides[:-1]):
-            return t, strides[:-1]
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()[:-1]
+    return t, strides[:-1]
 
 
 def _span(t: torch.Tensor):

@@ -145,3 +145,17 @@ def test_status_word_of_another_type():
     from gpa_vggt_b200 import kernels
     with pytest.raises(ValueError, match="status"):
         kernels.attention_shared_prefix(*_args(), status=torch.zeros(1))
+
+
+def test_strides_that_say_nothing():
+    """A dim of one entry, or any dim of an empty tensor, may have any stride; the
+    C entry takes multiples of 8 and must not see it."""
+    from gpa_vggt_b200 import kernels
+    odd = torch.zeros(2, 4 * 8 * 64 + 3, dtype=BF16)[:, :4 * 8 * 64].view(2, 4, 8, 64)[1:]
+    first = torch.zeros(2 * 8 * 4 * 8 * 64, dtype=BF16)[:4 * 8 * 64].as_strided((1, 4, 8, 64), (7, 512, 64, 1))
+    empty = torch.zeros(2, 2, 10, 68, dtype=BF16)[:, :, :0, :64]
+    for t in (first, empty):
+        assert t.is_contiguous()
+        u, strides = kernels._vectors(t)
+        assert u is t and not any(s % 8 for s in strides)
+    assert odd.is_contiguous() and not any(s % 8 for s in kernels._vectors(odd)[1])   # (its base is odd: copied)

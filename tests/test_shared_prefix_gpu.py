@@ -466,3 +466,29 @@ def test_more_query_heads_than_a_tile_has_rows(size):
 ])
 def test_every_width_of_the_join(size, own_len):
     check(make(*size, bias="key" if size[5] else None, own_len=own_len, causal=True, seed=6))
+
+
+@pytest.mark.parametrize("M", [1, 300])
+def test_strides_that_say_nothing(M):
+    """One request, and no prefix or cache at all, cut out of buffers whose rows lie an
+    odd number of values apart."""
+    a = make(1, M, 4, 2, 64, 3000, 200, bias="key", seed=12)
+    g = torch.Generator(device="cuda").manual_seed(13)
+
+    def odd(t):
+        buf = torch.randn(t.numel() + 16, device="cuda", generator=g).bfloat16()[:t.numel()]
+        view = buf.as_strided(t.shape, (t.numel() + 3, *t.stride()[1:]))
+        view.copy_(t)
+        return view
+    for name in ("q", "k_own", "v_own"):
+        a[name] = odd(a[name])
+        assert a[name].stride(0) % 8 and a[name].is_contiguous()
+    out = odd(torch.zeros(1, 4, M, 64, device="cuda", dtype=BF16))
+    got = run(a, out=out)
+    check(a, got)
+    wide = torch.zeros(1, 2, 200, 68, device="cuda", dtype=BF16)[:, :, :0, :64]
+    a["k_own"], a["v_own"] = wide, wide
+    check(a)
+    a = make(1, M, 4, 2, 64, 0, 200, seed=12)
+    a["k_prefix"], a["v_prefix"] = wide[0], wide[0]
+    check(a)

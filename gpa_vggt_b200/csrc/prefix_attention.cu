@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t swz(int row, int c) {
 // A prefix bias in log2 units.  -inf (or NaN) takes the key out; the type's
 // lowest values stay finite, so keys that all carry them are still weighed.
 __device__ __forceinline__ float bias_log2(float b) {
-  return b > -INFINITY ? fminf(fmaxf(b * 1.4426950408889634f, -3.402823466e38f), 3.402823466e38f) : -INFINITY;
+  return b > -INFINITY ? fminf(fmaxf(b, -kBiasLimit), kBiasLimit) * 1.4426950408889634f : -INFINITY;
 }
 
 // Tokens are counted through all requests (prefix) or within one (own).

@@ -49,6 +49,11 @@ __device__ __forceinline__ int query_count(const Params& p, int r) {
   return p.q_len ? min(max(__ldg(p.q_len + r), 0), p.queries) : p.queries;
 }
 
+// Finite biases count as at most this much, either way.  Both kernels keep it: at
+// every scale that tc_kernel takes, the bias over the scale stays inside fp32.
+constexpr float kBiasLimit = 1e30f;
+constexpr float kLeastScale = 1e-6f, kMostScale = 1e6f;
+
 // What the sum of a row's first partial output holds when its output is written.
 constexpr float kWritten = -1.0f;
 

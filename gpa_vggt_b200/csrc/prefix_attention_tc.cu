@@ -43,11 +43,13 @@ namespace prefix {
 constexpr int TC_THREADS = 384;
 constexpr int TM = 128;   // rows and keys per tile
 constexpr int XTILE = TM * 16 * 2;
-// Finite biases end here (log2 units).  A row of nothing but the type's lowest
-// value spreads evenly: scores up to 64 vanish beside 2^30, and c*x - c*m, off by
-// the rounding of c*m (at most 64, the same for all of a row's keys), stays inside
-// the exponent's range.
-constexpr float kBiasLimit = 1073741824.f;
+// c*x - c*m is off by the rounding of c*m, the same for all of a row's keys.  Up to
+// this maximum (log2 units) that is at most 64 and stays inside the exponent's range.
+// Beyond it (large biases, or nothing but the type's lowest value) scores that differ
+// at all differ by 64 or more, so that only keys at the maximum count, and any factor
+// near c gives the same weights: such a row takes c's power of two, whose products are
+// exact.  (Taking m off x first costs every row: 612 us for 549 at 4 x 1,374 tokens.)
+constexpr float kFar = 1073741824.f;
 constexpr int TC_REGS = 168, TC_LOW = 80, TC_HIGH = 208;
 static_assert(TC_LOW * 128 + TC_HIGH * 256 <= TC_REGS * TC_THREADS, "register split");
 
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int row = lane; row < TM; row += 32)   // 1, 1, 1, 0, ...
         *reinterpret_cast<uint2*>(smem + SM::ONES + xtile_off(row, 0)) = make_uint2(0x3F803F80u, 0x3F80u);
       fence_async_smem();
-      const float inv_scale = 1.0f / p.scale, most = kBiasLimit / p.scale_log2;
+      const float inv_scale = 1.0f / p.scale, most = kBiasLimit * inv_scale;
       int i = 0, gk = 0, gv = 0;
       bool okw = true;
       Piece c;
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t tS = tbase + lane_off + col_s(t), tO = tbase + lane_off + col_o(t), tP = tbase + lane_off + col_p(t);
     float2* half_ml = reinterpret_cast<float2*>(smem + SM::ML) + row_i;
-    const float c2 = p.scale_log2;
+    const float c2 = p.scale_log2, c2_pow2 = __uint_as_float(__float_as_uint(c2) & 0x7f800000u);
     constexpr float kNoMax = -3.0e38f;   // no key yet
     int cs = 0, g = 0, ih = 0;   // ih: pieces in halves so far
     bool okw = true;
@@ -619,13 +621,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       const bool idle = !__any_sync(0xffffffffu, live);   // a warp without rows only keeps the barriers going
       float m_raw = kNoMax, l = 0.f;       // running maximum (score units), row sum
-      float neg_mc = 0.f;                  // -c2 * m_raw
-      auto quarter = [&](float* xq, float neg, float* acc, uint32_t* pk) {
+      float cr = c2, neg_mc = 0.f;         // the row's factor, and -cr * m_raw
+      // For each tile at head_dim 64, where the maximum moves at 128: the other way round
+      // four frames take 577 us for 549, 9,472 rows x 16,384 keys 740 for 693 at 128.
+      auto set_factor = [&] {
+        cr = fabsf(m_raw * c2) > kFar ? c2_pow2 : c2;
+        neg_mc = -m_raw * cr;
+        if (D == 64) neg_mc = fminf(neg_mc, -kNoMax);   // of a row without a key yet: finite
+      };
+      auto quarter = [&](float* xq, float* acc, uint32_t* pk) {
 #pragma unroll
         for (int e8 = 0; e8 < 4; ++e8) {
           float* xg = xq + e8 * 8;
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) ffma2(xg[i], xg[i + 1], xg[i], xg[i + 1], c2, c2, neg, neg);
+          for (int i = 0; i < 8; i += 2) ffma2(xg[i], xg[i + 1], xg[i], xg[i + 1], cr, cr, neg_mc, neg_mc);
           float e[8];
           exp8(xg, e);
 #pragma unroll
@@ -681,14 +690,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             alpha = fast_exp2((m_raw - mt) * c2);
             l = mt < INFINITY ? l * alpha : NAN;   // a NaN or infinite score: the row is NaN (the polynomial would lose it)
             m_raw = mt < INFINITY ? mt : 0.f;
-            neg_mc = -m_raw * c2;
+            if (D == 128) set_factor();
           }
         }
+        if (D == 64) set_factor();
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         uint32_t pk[4][16];
 #pragma unroll
         for (int qt = 0; qt < 4; ++qt) {
-          quarter(x + qt * 32, neg_mc, acc, pk[qt]);
+          quarter(x + qt * 32, acc, pk[qt]);
           if (D == 128) {   // S(j) came after O += P(j-1) V
             tmem_st16(tP + qt * 16, pk[qt]);
           } else if (qt == 1) {
@@ -843,7 +853,7 @@ static bool stride_ok(int64_t n, int64_t s) { return n <= 1 || (s > 0 && s < (1l
 
 bool tc_takes(const Params& p, int head_dim, bool fold) {
   // the maximum is taken on unscaled scores, and the bias divided by the scale
-  if (!(p.scale > 1e-6f && p.scale < 1e6f) || p.group > TM) return false;
+  if (!(p.scale > kLeastScale && p.scale < kMostScale) || p.group > TM) return false;
   if (!stride_ok(p.heads, p.q_sh) || !stride_ok(p.queries, p.q_sm) || !stride_ok(p.requests, p.q_sr)) return false;
   if (fold && p.requests > 1 && p.queries > 1 && p.q_sr != p.queries * p.q_sm) return false;
   if (p.prefix && (!stride_ok(p.kv_heads, p.kp_sh) || !stride_ok(p.prefix, p.kp_sn) || !stride_ok(p.kv_heads, p.vp_sh) ||

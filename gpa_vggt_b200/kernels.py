@@ -562,8 +562,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     Hk (H/Hk query heads in a row share a key head).  own_len, q_len: int32 [R]
     on the device (clamped to [0,N] and [0,M]), or None for all N and M; cache
     rows past own_len may hold anything.  bias: [P], [1,P] or [Hk,P], natural-log
-    domain; -inf (or NaN) takes a key out, whatever its K and V hold.  causal:
-    query i sees own keys j <= own_len - q_len + i, and every prefix key.
+    domain; -inf (or NaN) takes a key out, whatever its K and V hold; finite ones
+    count as at most 1e30 either way.  causal: query i sees own keys j <= own_len - q_len + i, and every prefix key.
 
     Returns out [R,H,M,D] bf16, and with return_lse (or lse_out) the log2 row
     sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len

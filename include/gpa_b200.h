@@ -437,7 +437,8 @@ GPA_API int gpa_residual_norm_backward(
  * each with its element strides (multiples of 8, innermost contiguous, 16-byte
  * aligned).  heads % kv_heads == 0: heads/kv_heads query heads in a row share
  * a key head.  head_dim 64 or 128.  bias: fp32 rows at bias + kv_head*bias_sh,
- * or NULL; -inf (or NaN) takes the key out, whatever its K and V hold.
+ * or NULL; -inf (or NaN) takes the key out, whatever its K and V hold; finite
+ * ones count as at most 1e30 either way.
  * own_len, q_len: device int32 [requests], or NULL for cache and queries;
  * read by the kernels, clamped to [0, cache] and [0, queries].  Cache rows past
  * own_len may hold anything.  Query rows past q_len are neither computed nor

@@ -492,3 +492,69 @@ def test_strides_that_say_nothing(M):
     a = make(1, M, 4, 2, 64, 0, 200, seed=12)
     a["k_prefix"], a["v_prefix"] = wide[0], wide[0]
     check(a)
+
+
+EVERY_KERNEL = [                        # sizes at which each kernel, and each form of it, runs
+    (2, 1, 4, 2, 64, 700, 40), (3, 30, 2, 2, 128, 700, 40),
+    (5, 300, 4, 4, 64, 3000, 500), (3, 260, 4, 4, 128, 3000, 500),       # joint, pairs of row tiles
+    (2, 128, 8, 8, 64, 5000, 300), (3, 100, 4, 4, 128, 7000, 200),       # joint, in halves
+    (16, 17, 8, 8, 64, 9000, 90), (100, 1, 16, 16, 64, 9000, 33),        # folded
+]
+
+
+@pytest.mark.parametrize("size", EVERY_KERNEL)
+def test_large_biases(size):
+    """The largest bias wins, however large: a row is its key's value, whichever kernel
+    runs.  Beyond 1e30 biases are alike."""
+    R, Hk, P = size[0], size[3], size[5]
+    g = torch.Generator(device="cuda").manual_seed(21)
+
+    def best(a, k, v):
+        """Key k of a head's prefix alone counts; its bias is v."""
+        out, lse = run(a)
+        want = torch.stack([a["v_prefix"][i, k[i]] for i in range(Hk)]).repeat_interleave(size[2] // Hk, 0)
+        assert torch.equal(out, want[None, :, None].expand_as(out))
+        # a bias is rounded to fp32 (on the tensor cores over the scale), and the score with it
+        assert bool(((lse.double() - v * math.log2(math.e)).abs() <= 2.0 ** -21 * abs(v) * math.log2(math.e)).all())
+
+    for low, high, own in [(1e9, 2e9, None), (1e6, 4e9, None), (-2e9, -1e9, 0), (-1e30, -1e12, 0), (1e29, 9e29, None)]:
+        for place in (0, P // 2, P - 1):
+            a = make(*size, bias="head", own_len=None if own is None else [own] * R, seed=22)
+            k = [(place + 131 * i) % P for i in range(Hk)]
+            a["bias"] = low * (1 + torch.rand(Hk, P, device="cuda", generator=g) / (4 if low > 0 else -4))
+            a["bias"][torch.arange(Hk), k] = high
+            best(a, k, high)
+    for side in (1, -1):
+        a = make(*size, bias="head", own_len=[0] * R, seed=23)
+        a["bias"].fill_(-INF)
+        top = torch.tensor([1e31, 1e30, torch.finfo(F32).max, 5e33], device="cuda") * side
+        a["bias"][:, [3, P // 2, P - 2, P - 1]] = top
+        out, _ = run(a)
+        v = a["v_prefix"][:, [3, P // 2, P - 2, P - 1]].double().repeat_interleave(size[2] // Hk, 0)
+        mean, mag = v.mean(1)[None, :, None], v.abs().mean(1)[None, :, None]
+        assert bool(((out.double() - mean).abs() <= H8 * (mean.abs() + mag) + 2.0 ** -10 * mag).all())
+
+
+@pytest.mark.parametrize("size", EVERY_KERNEL)
+@pytest.mark.parametrize("scale", [0.125, 16.0])
+def test_exact_scores_that_move_the_maximum(size, scale):
+    """Small whole numbers in q and k: the scores, up to some thousands, are exact in
+    fp32, so the ordinary bounds hold; later keys score higher, so the maximum moves
+    often, and the first keys are out, so rows begin without one."""
+    R, M, H, Hk, D, P, N = size
+    g = torch.Generator(device="cuda").manual_seed(31)
+
+    def whole(*s):
+        return torch.randint(-1, 2, s, device="cuda", generator=g).to(BF16)
+    for causal in (False, True):
+        a = make(*size, bias="head", own_len=[(37 * r) % (N + 1) for r in range(R)], causal=causal, seed=32)
+        a["sm_scale"] = scale
+        a["q"] = whole(R, H, M, D)
+        for name, n in (("k_prefix", P), ("k_own", N)):
+            grow = 1 + 6 * torch.arange(n, device="cuda")[:, None] // n
+            a[name] = whole(*a[name].shape) * grow.to(BF16)
+        a["bias"] = torch.randint(0, 4, (Hk, P), device="cuda", generator=g).float() * scale
+        a["bias"][:, :P // 3] = -INF
+        check(a)
+        a["bias"].fill_(-INF)                   # the caches alone, some of them empty
+        check(a)

@@ -12,6 +12,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, ptr, stream_of, require_cuda, aligned
@@ -127,6 +128,13 @@ def _one_device(first: torch.Tensor, *others, what: str) -> int:
             require_cuda(t, what=what)
             raise ValueError(f"{what}: tensors are on different devices")
     return index
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of them carries a forward-mode derivative, which a kernel that
+    works on addresses would drop without a word."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _on(index: int):
@@ -543,6 +551,8 @@ def _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bi
         for t in (q, k_prefix, v_prefix, k_own, v_own, bias):
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: no gradients (call it under torch.no_grad())")
+    if has_tangent(q, k_prefix, v_prefix, k_own, v_own, bias):
+        raise ValueError(f"{what}: no forward-mode derivatives")
     return _one_device(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status, what=what)
 
 
@@ -569,7 +579,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
     -inf.  `out` and `lse_out` lie outside the inputs' memory.  Nothing is read back to the host, so calls can be captured; no
-    gradients.  Many rows per key head run on the tensor cores, few as a stream of
+    gradients, backward or forward-mode.  Many rows per key head run on the tensor cores, few as a stream of
     the keys (the choice is by sizes and strides, not by values); a pipeline wait
     that gives up is recorded in the device's status word (check_device_status)."""
     index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status)
@@ -856,6 +866,8 @@ def _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind,
         if len(g) < 1 or g[-1] != C or (len(g) > 1 and not _leads(g[:-1], shape[:-1])):
             raise ValueError("residual_norm: gate must be [C], or x's shape with trailing dims before the "
                              "last of size 1 ([B, 1, C], [B, N, C])")
+    if has_tangent(x, y, gate, weight, bias, post_weight, post_bias):
+        raise ValueError("residual_norm: no forward-mode derivatives")
     _one_device(x, y, gate, weight, bias, post_weight, post_bias, what="residual_norm")
 
 
@@ -886,7 +898,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor]
     parameters are all bf16 or all fp32.  fp32 arithmetic; for a bf16 stream the
     roundings are those of residual_scale and layernorm one after the other.
     C % 8 == 0, C <= 8192.  Differentiable once in x, y, gate and the norm
-    parameters; column sums run in a fixed order."""
+    parameters (backward; forward-mode derivatives are refused); column sums run
+    in a fixed order."""
     _check_residual_norm(x, y, gate, weight, bias, post_weight, post_bias, kind, post_kind)
     if torch.is_grad_enabled():
         for t in (x, y, gate, weight, bias, post_weight, post_bias):

@@ -83,3 +83,17 @@ def test_workspace_covers_every_worker(lib):
                 n = lib.gpa_residual_norm_backward_workspace_bytes(rows, cols, gate_rows)
                 workers, rest = divmod(n, 5 * cols * 4)
                 assert rest == 0 and 1 <= workers <= min(rows, 2 * 148 * 16)
+
+
+@pytest.mark.parametrize("name", ["x", "y", "gate", "weight", "bias", "post_weight", "post_bias"])
+def test_forward_mode_derivatives_are_refused(name):
+    from torch.autograd import forward_ad
+    from gpa_vggt_b200 import kernels
+    t = dict(x=_t(2, 16, dtype=F32), y=_t(2, 16, dtype=F32),
+             **{k: _t(16, dtype=F32) for k in ("gate", "weight", "bias", "post_weight", "post_bias")})
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="CUDA device"):       # no tangent: refused for the CPU alone
+            kernels.residual_norm(**t, post_kind="layer")
+        t[name] = forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+        with pytest.raises(ValueError, match="residual_norm: no forward-mode"):
+            kernels.residual_norm(**t, post_kind="layer")

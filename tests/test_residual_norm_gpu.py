@@ -405,3 +405,22 @@ def test_block_calls_a_norm_that_someone_watches(how):
             block.norm2.__class__ = Watched
         out = block(x)
     assert seen == [x.shape] and torch.equal(out, ref)
+
+
+def test_forward_mode_derivatives():
+    """residual_norm refuses a dual tensor aloud; Block, whose kernels know no
+    derivatives, keeps its values."""
+    from torch.autograd import forward_ad
+    from gpa_vggt_b200.vggt import layers
+    t = make((2, 9, 256), BF16, BF16, BF16, "channel", "layer", None)
+    torch.manual_seed(2)
+    block = layers.Block(256, 4, init_values=0.3, qk_norm=True).cuda().bfloat16().eval()
+    with torch.no_grad():
+        ref = block(t["x"])
+    with forward_ad.dual_level(), torch.no_grad():
+        assert torch.equal(call(t, "layer", None)[0], call(t, "layer", None)[0])
+        dual = forward_ad.make_dual(t["x"], torch.ones_like(t["x"]))
+        assert torch.equal(forward_ad.unpack_dual(block(dual)).primal, ref)
+        t["x"] = dual
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(t, "layer", None)

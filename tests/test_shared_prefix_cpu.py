@@ -159,3 +159,19 @@ def test_strides_that_say_nothing():
         u, strides = kernels._vectors(t)
         assert u is t and not any(s % 8 for s in strides)
     assert odd.is_contiguous() and not any(s % 8 for s in kernels._vectors(odd)[1])   # (its base is odd: copied)
+
+
+@pytest.mark.parametrize("i", [0, 1, 2, 3, 4, "bias"])
+def test_forward_mode_derivatives_are_refused(i):
+    from torch.autograd import forward_ad
+    from gpa_vggt_b200 import kernels
+    args, bias = _args(), torch.zeros(5)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="CUDA device"):       # no tangent: refused for the CPU alone
+            kernels.attention_shared_prefix(*args, bias=bias)
+        if i == "bias":
+            bias = forward_ad.make_dual(bias, torch.ones(5))
+        else:
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+        with pytest.raises(ValueError, match="attention_shared_prefix: no forward-mode"):
+            kernels.attention_shared_prefix(*args, bias=bias)

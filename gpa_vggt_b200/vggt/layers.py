@@ -501,7 +501,8 @@ def _residual_norm(x, ls, y, norm):
             and y.dtype == BF16 and ls.gamma.dtype == BF16 and x.shape == y.shape
             and norm.weight is not None and norm.bias is not None and C in (256, 512, 1024, 2048)
             and _unhooked(norm) and not kernels.has_tangent(x, y, ls.gamma, norm.weight, norm.bias)):
-        return kernels.residual_norm(x, y, ls.gamma, norm.weight, norm.bias, norm.eps)
+        with torch.no_grad():   # as in the kernels before and after it: they have no gradients to pass on
+            return kernels.residual_norm(x, y, ls.gamma, norm.weight, norm.bias, norm.eps)
     x = _residual(x, ls, y)
     return x, norm(x)
 

@@ -424,3 +424,18 @@ def test_forward_mode_derivatives():
         t["x"] = dual
         with pytest.raises(ValueError, match="forward-mode"):
             call(t, "layer", None)
+
+
+def test_block_keeps_nothing_for_gradients():
+    """Block's other bf16 kernels have no gradients, so no part of a graph is built
+    (and no z, y and statistics kept) for it with gradients enabled."""
+    from gpa_vggt_b200.vggt import layers
+    torch.manual_seed(3)
+    block = layers.Block(256, 4, init_values=0.3, qk_norm=True).cuda().bfloat16().eval()
+    x = torch.randn(2, 33, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        ref = block(x)
+    seen = []
+    block.mlp.register_forward_pre_hook(lambda m, i: seen.append(i[0].requires_grad))
+    out = block(x.requires_grad_(True))
+    assert seen == [False] and not out.requires_grad and torch.equal(out, ref)

@@ -495,10 +495,12 @@ def _unhooked(norm):
 
 def _residual_norm(x, ls, y, norm):
     """(x + ls(y), norm of it).  Where _residual and LayerNorm both take their
-    fused kernels this is one pass with the same results, bit for bit."""
+    fused kernels this is one pass with the same results, bit for bit: at the
+    widths of layernorm's kernel up to 2,048 (its fifth, 4,096, sums in another
+    order), and a gamma of one dim (residual_scale takes any shape of C values)."""
     C = x.shape[-1]
     if (isinstance(ls, LayerScale) and isinstance(norm, LayerNorm) and x.is_cuda and x.dtype == BF16
-            and y.dtype == BF16 and ls.gamma.dtype == BF16 and x.shape == y.shape
+            and y.dtype == BF16 and ls.gamma.dtype == BF16 and ls.gamma.dim() == 1 and x.shape == y.shape
             and norm.weight is not None and norm.bias is not None and C in (256, 512, 1024, 2048)
             and _unhooked(norm) and not kernels.has_tangent(x, y, ls.gamma, norm.weight, norm.bias)):
         with torch.no_grad():   # as in the kernels before and after it: they have no gradients to pass on

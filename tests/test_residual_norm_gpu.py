@@ -439,3 +439,16 @@ def test_block_keeps_nothing_for_gradients():
     block.mlp.register_forward_pre_hook(lambda m, i: seen.append(i[0].requires_grad))
     out = block(x.requires_grad_(True))
     assert seen == [False] and not out.requires_grad and torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("shape", [(1, 256), (256, 1), (1, 1, 256), (1, 1, 1, 256)])
+def test_block_with_a_gamma_of_more_dims(shape):
+    """LayerScale's kernel takes any gamma of C values, and so does Block."""
+    from gpa_vggt_b200.vggt import layers
+    torch.manual_seed(4)
+    block = layers.Block(256, 4, init_values=0.3, qk_norm=True).cuda().bfloat16().eval()
+    x = torch.randn(2, 33, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        ref = block(x)
+        block.ls1.gamma = torch.nn.Parameter(block.ls1.gamma.reshape(shape))
+        assert torch.equal(block(x), ref)

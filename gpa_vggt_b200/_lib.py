@@ -77,6 +77,7 @@ SIGNATURES = {
                                             _vp, _c_int, _vp, _c_int, _vp, _c_i64, _vp, _c_i64, _vp, _vp,
                                             _vp, _vp, _vp, _vp, _c_i64, _vp]),
     "gpa_attention_shared_prefix_workspace_bytes": (_c_i64, [_c_int] * 7),
+    "gpa_attention_shared_prefix_call_bytes": (_c_i64, [_c_i64] * 13 + [_c_int] * 7 + [_c_f32]),
     "gpa_attention_shared_prefix": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64,
                                              _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64,
                                              _c_i64, _c_i64, _vp, _vp] + [_c_int] * 7 + [_c_f32, _c_int, _vp,

@@ -505,6 +505,8 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const T
   const float2* tml = p.tc_ml + (int64_t)block * 128 + i;
   const int64_t tstep = (int64_t)tc.blocks * 128;
   const float2 first = tml[0];
+  // part s is the CTA's that begins the item, or of one behind it (inside the grid, whatever a wait that gave up left)
+  const int cta0 = max(p.tc_first[block], 0);
   if (first.y == kWritten) return;
   const int64_t row = row_index(p, w);
   const int slots = p.s1 + p.s2;
@@ -531,7 +533,7 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const T
       v[4 * u + 3] = fmaf(f, x[u].w, v[4 * u + 3]);
     }
   };
-  auto join = [&](int n, const float2* ml, int64_t ml_step, const float4* o, int64_t o_step, auto f_step) {
+  auto join = [&](int n, const float2* ml, int64_t ml_step, auto o, auto f_step) {   // o(s): part s's features
     if constexpr (FEW) {
       constexpr int AHEAD = 8;
       for (int s0 = 0; s0 < n; s0 += AHEAD) {
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const T
         for (int a = 0; a < AHEAD; ++a)
 #pragma unroll
           for (int u = 0; u < F / 4; ++u)
-            x[a][u] = f[a] > 0.f ? o[(s0 + a) * o_step + u * f_step] : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[a][u] = f[a] > 0.f ? o(s0 + a)[u * f_step] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) add(f[a], x[a]);
       }
@@ -555,16 +557,19 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const Params p, const T
         if (f > 0.f) {
           float4 x[F / 4];
 #pragma unroll
-          for (int u = 0; u < F / 4; ++u) x[u] = o[s * o_step + u * f_step];
+          for (int u = 0; u < F / 4; ++u) x[u] = o(s)[u * f_step];
           add(f, x);
         }
       }
     }
   };
-  join(tc.slots, tml, tstep, p.tc_o + ((int64_t)block * (D / 4) + f0 / 4) * 128 + i, (int64_t)tc.blocks * (D / 4) * 128,
+  const int second = tc.halves ? 0 : (block - rk * tc.tiles) & 1;
+  const float4* to = p.tc_o + f0 / 4 * 128 + i;
+  join(tc.slots, tml, tstep,
+       [&](int s) { return to + part_tile(tc, block, second, min(cta0 + s, tc.ctas - 1), s == 0) * (D / 4 * 128); },
        std::integral_constant<int, 128>());
-  join(slots, p.ws_ml + row, p.rows, reinterpret_cast<const float4*>(p.ws_o + row * D + f0), p.rows * (D / 4),
-       std::integral_constant<int, 1>());
+  const float4* wo = reinterpret_cast<const float4*>(p.ws_o + row * D + f0);
+  join(slots, p.ws_ml + row, p.rows, [&](int s) { return wo + s * p.rows * (D / 4); }, std::integral_constant<int, 1>());
   const float inv = l == 0.f ? 0.f : 1.f / l;   // no key: zero (a NaN stays one)
   uint4* dst = reinterpret_cast<uint4*>(p.o + w.r * p.o_sr + w.h * p.o_sh + w.m * p.o_sm + f0);
 #pragma unroll
@@ -598,8 +603,9 @@ struct Plan {
   int wm1, rt1, s1, wm2, rt2, s2, chunk;
   int64_t items, rows;
   TcPlan tc;
-  int64_t floats(int head_dim) const {   // of the partial outputs
-    return (tc_run ? (int64_t)tc.slots * tc.blocks * 128 * (head_dim + 2) : 0) + (s1 + s2) * rows * (head_dim + 2);
+  int64_t bytes(int head_dim) const {   // of the partial outputs, in whole ones of a row
+    const int64_t tiles = tc_run ? part_tiles(tc) * 128 * head_dim + (int64_t)tc.blocks * (tc.slots * 256 + 1) : 0;
+    return ((tiles + head_dim + 1) / (head_dim + 2) + (s1 + s2) * rows) * (head_dim + 2) * 4;
   }
 };
 
@@ -692,6 +698,7 @@ static Plan make_plan(int requests, int queries, int heads, int kv_heads, int he
     p.s2 = (int)((t2 + per - 1) / per);
     p.items = kv_heads * ((int64_t)p.rt1 * p.s1 + (int64_t)requests * p.rt2 * p.s2);
   }
+  p.tc.keep = p.tc_run && p.s2 > 0;
   return p;
 }
 
@@ -765,9 +772,29 @@ extern "C" int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int
   // strides decide which kernels can run: room for each way
   int64_t bytes = 0;
   for (int way = 0; way < 4; ++way)
-    bytes = std::max(bytes, 4 * prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache, way & 1,
-                                                  way & 2).floats(head_dim));
+    bytes = std::max(bytes, prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix, cache, way & 1,
+                                              way & 2).bytes(head_dim));
   return bytes;
+}
+
+extern "C" int64_t gpa_attention_shared_prefix_call_bytes(
+    int64_t q_sr, int64_t q_sh, int64_t q_sm, int64_t kp_sh, int64_t kp_sn, int64_t vp_sh, int64_t vp_sn, int64_t ko_sr,
+    int64_t ko_sh, int64_t ko_sn, int64_t vo_sr, int64_t vo_sh, int64_t vo_sn, int requests, int queries, int heads,
+    int kv_heads, int head_dim, int prefix_len, int cache_len, float sm_scale) {
+  if (prefix::check_sizes("gpa_attention_shared_prefix_call_bytes", requests, queries, heads, kv_heads, head_dim,
+                          prefix_len, cache_len))
+    return -1;
+  if (requests == 0 || queries == 0) return 0;
+  prefix::Params p{};
+  p.requests = requests; p.queries = queries; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
+  p.prefix = prefix_len; p.cache = cache_len;
+  p.q_sr = q_sr; p.q_sh = q_sh; p.q_sm = q_sm;
+  p.kp_sh = kp_sh; p.kp_sn = kp_sn; p.vp_sh = vp_sh; p.vp_sn = vp_sn;
+  p.ko_sr = ko_sr; p.ko_sh = ko_sh; p.ko_sn = ko_sn;
+  p.vo_sr = vo_sr; p.vo_sh = vo_sh; p.vo_sn = vo_sn;
+  p.scale = sm_scale;
+  return prefix::make_plan(requests, queries, heads, kv_heads, head_dim, prefix_len, cache_len,
+                           prefix::tc_takes(p, head_dim, false), prefix::tc_takes(p, head_dim, true)).bytes(head_dim);
 }
 
 extern "C" int gpa_attention_shared_prefix(
@@ -823,18 +850,18 @@ extern "C" int gpa_attention_shared_prefix(
                         prefix::tc_takes(p, head_dim, false), prefix::tc_takes(p, head_dim, true));
   if (plan.items >= (1ll << 31))
     return fail(GPA_ERR_UNSUPPORTED, "%s: too many work items", what);
-  const int64_t bytes = 4 * plan.floats(head_dim);
+  const int64_t bytes = plan.bytes(head_dim);
   if (bytes && (!workspace || !aligned16(workspace) || workspace_bytes < bytes))
     return fail(GPA_ERR_INVALID, "%s: workspace missing, unaligned or too small", what);
   p.status = status;
   p.rt1 = plan.rt1; p.s1 = plan.s1; p.rt2 = plan.rt2; p.s2 = plan.s2; p.chunk = plan.chunk;
   p.rows = plan.rows;
-  // the tiles' outputs (whole lines each), the rows', then their maxima and sums
-  const int64_t tile_rows = plan.tc_run ? (int64_t)plan.tc.slots * plan.tc.blocks * 128 : 0;
+  // the tiles' outputs (whole lines each), the rows', their maxima and sums, then the items' first CTAs
   p.tc_o = (float4*)workspace;
-  p.ws_o = (float*)workspace + tile_rows * head_dim;
+  p.ws_o = (float*)workspace + (plan.tc_run ? prefix::part_tiles(plan.tc) * 128 * head_dim : 0);
   p.tc_ml = reinterpret_cast<float2*>(p.ws_o + (plan.s1 + plan.s2) * plan.rows * head_dim);
-  p.ws_ml = p.tc_ml + tile_rows;
+  p.ws_ml = p.tc_ml + (plan.tc_run ? (int64_t)plan.tc.slots * plan.tc.blocks * 128 : 0);
+  p.tc_first = reinterpret_cast<int32_t*>(p.ws_ml + (plan.s1 + plan.s2) * plan.rows);
   cudaStream_t st = (cudaStream_t)stream;
   return head_dim == 64 ? prefix::launch<64>(p, plan, st) : prefix::launch<128>(p, plan, st);
 }

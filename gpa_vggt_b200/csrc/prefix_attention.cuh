@@ -27,8 +27,9 @@ struct Params {
   float2* ws_ml;                 // [s1 + s2][rows]: maximum (log2 units) and sum
   // tc_kernel's: a row tile's outputs lie feature group by feature group, so that
   // its threads, one per row, write and read whole lines
-  float4* tc_o;                  // [slots][blocks][D / 4][128 rows]
+  float4* tc_o;                  // [part_tiles(tc)][D / 4][128 rows], see part_tile
   float2* tc_ml;                 // [slots][blocks][128 rows]
+  int32_t* tc_first;             // [blocks]: the CTA that begins the item
   int* status;
 };
 
@@ -74,7 +75,23 @@ struct TcPlan {
   int ctas;      // each takes a span of the units of work
   int least;     // of at least so many: no item is cut into more than `slots` parts
   int slots;
+  int keep;      // chunks of rows_kernel join in: also items that are not cut leave their outputs,
+                 // two fp32 rows for each of bf16 (200 x 1,374 tokens over 66,845 + 1,374 keys: 2.4 GB and
+                 // 109 ms; the joint form would take 0.1 GB and 118 ms)
 };
+
+// Where the output of an item's part lies.  A CTA's span begins inside at most one
+// item and ends inside at most one, so that its parts have two places (and two row
+// tiles each), whatever the number of rows; `first` parts lie by row tile where
+// uncut items leave theirs too.
+__host__ __device__ inline int64_t part_tiles(const TcPlan& tc) {
+  return (tc.keep ? tc.blocks : tc.ctas * (tc.halves ? 1 : 2)) + (int64_t)tc.ctas * (tc.halves ? 1 : 2);
+}
+__device__ __forceinline__ int64_t part_tile(const TcPlan& tc, int block, int second, int cta, bool first) {
+  if (tc.keep && first) return block;
+  const int per = tc.halves ? 1 : 2;
+  return (tc.keep ? tc.blocks : first ? tc.ctas * per : 0) + (int64_t)cta * per + second;
+}
 
 // Row i of row tile `block` of tc_kernel.
 __device__ __forceinline__ Row tile_row(const Params& p, const TcPlan& tc, int kh, int req, int tile, int i) {

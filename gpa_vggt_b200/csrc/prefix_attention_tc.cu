@@ -770,6 +770,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       // the row tile among the partial outputs, and in this piece's slot
       const int block = (c.req * p.kv_heads + c.kh) * tc.tiles + c.tile + (HALVES ? 0 : t);
       const int64_t to = (int64_t)c.slot * tc.blocks + block;
+      const int64_t part = part_tile(tc, block, HALVES ? 0 : t, blockIdx.x, c.first);
       __nv_bfloat16* orow = p.o + row.r * p.o_sr + row.h * p.o_sh + row.m * p.o_sm;
       if (!idle) {
 #pragma unroll
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             for (int i = 0; i < 4; ++i)
               reinterpret_cast<uint4*>(orow + u * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           } else if (some) {
-            float4* w = p.tc_o + (to * (D / 4) + u * 8) * TM + row_i;
+            float4* w = p.tc_o + (part * (D / 4) + u * 8) * TM + row_i;
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i * TM] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
@@ -810,6 +811,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(half_read);
       }
+      // (a second tile without rows is another item's, or none)
+      if (c.first && !direct && row_i == 0 && (HALVES || t == 0 || !c.single)) p.tc_first[block] = blockIdx.x;
       if (row.live) {
         if (direct) {
           if (p.lse) p.lse[row.r * p.lse_sr + row.h * p.lse_sh + row.m] = some ? m_raw * c2 + log2f(l) : -INFINITY;

@@ -607,7 +607,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         if bias.dim() == 2 and bias.shape[0] > 1:
             bias_sh = bias.stride(0)
     own_len, q_len = (None if t is None else t.contiguous() for t in (own_len, q_len))
-    size = _lib.load().gpa_attention_shared_prefix_workspace_bytes(R, M, H, Hk, D, P, N)
+    size = _lib.load().gpa_attention_shared_prefix_call_bytes(*qs, *kps, *vps, *kos, *vos, R, M, H, Hk, D, P, N,
+                                                              sm_scale)
     ws = torch.empty(size, device=device, dtype=torch.uint8) if size > 0 else None
     status, own = _status_word(status, device)
     ls = (0, 0) if lse_out is None else lse_out.stride()[:2]

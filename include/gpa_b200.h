@@ -446,11 +446,16 @@ GPA_API int gpa_residual_norm_backward(
  * + i (the last query sees all); the prefix is seen by every query.  A query
  * without keys gives 0 and lse -inf.  lse: fp32, rows contiguous, or NULL.  o
  * and lse overlap no input.  status: device int, set to 1 where a pipeline wait
- * gives up, or NULL.  workspace: 16-byte aligned, _workspace_bytes() (-1: bad sizes); calls that may
- * overlap need their own.
+ * gives up, or NULL.  workspace: 16-byte aligned; calls that may overlap need their
+ * own.  _workspace_bytes() is enough for any strides and scale, _call_bytes() for a
+ * call with these (-1: bad sizes).
  */
 GPA_API int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int queries, int heads, int kv_heads,
                                                             int head_dim, int prefix, int cache);
+GPA_API int64_t gpa_attention_shared_prefix_call_bytes(
+    int64_t q_sr, int64_t q_sh, int64_t q_sm, int64_t kp_sh, int64_t kp_sn, int64_t vp_sh, int64_t vp_sn, int64_t ko_sr,
+    int64_t ko_sh, int64_t ko_sn, int64_t vo_sr, int64_t vo_sh, int64_t vo_sn, int requests, int queries, int heads,
+    int kv_heads, int head_dim, int prefix, int cache, float sm_scale);
 GPA_API int gpa_attention_shared_prefix(
     const void* q, int64_t q_sr, int64_t q_sh, int64_t q_sm, const void* k_prefix, int64_t kp_sh, int64_t kp_sn,
     const void* v_prefix, int64_t vp_sh, int64_t vp_sn, const float* bias, int64_t bias_sh, const void* k_own,

@@ -175,3 +175,51 @@ def test_forward_mode_derivatives_are_refused(i):
             args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
         with pytest.raises(ValueError, match="attention_shared_prefix: no forward-mode"):
             kernels.attention_shared_prefix(*args, bias=bias)
+
+
+def _call_bytes(lib, R, M, H, Hk, D, P, N, scale=0.125, q_sr=None):
+    """Contiguous token-major queries and caches, a head-major prefix."""
+    return lib.gpa_attention_shared_prefix_call_bytes(
+        M * H * D if q_sr is None else q_sr, D, H * D, P * D, D, P * D, D, N * Hk * D, D, Hk * D, N * Hk * D, D, Hk * D,
+        R, M, H, Hk, D, P, N, scale)
+
+
+@pytest.mark.parametrize("size,folded", [((64, 1374, 16, 16, 64, 16711, 1374), False),
+                                         ((200, 1374, 16, 16, 64, 66845, 1374), True),
+                                         ((40, 3000, 16, 4, 128, 5000, 3000), False),
+                                         ((8, 20000, 8, 8, 128, 0, 20000), False),
+                                         ((1, 274800, 16, 16, 64, 66845, 0), False)])
+def test_workspace_of_many_rows(lib, size, folded):
+    """Only items that a span's end cuts leave parts, at most two to a CTA: 20 MB at
+    head_dim 64, 39 at 128; beside them 8 bytes a row and part of its tile.  In a folded
+    call with caches the few-rows kernel's outputs of the caches join in, one fp32 row
+    of D + 2 values for each row (long calls cut no cache), and so every row tile of the
+    prefix leaves its own: 4 D bytes a row twice, for 2 D of output."""
+    R, M, H, Hk, D, P, N = size
+    n = _call_bytes(lib, *size)
+    out = R * M * H * D * 2
+    rows = 128 * -(-M // (128 // (H // Hk))) * R * Hk
+    copies = rows * 4 * D + R * M * H * 4 * (D + 2) if folded else 0
+    assert 0 < n <= 148 * 2 * 2 * 128 * D * 4 + 3 * (8 * rows + 4 * R * Hk * M) + (1 << 16) + copies
+    assert n < (40 << 20) + out // 4 + (copies if folded else 0)
+
+
+def test_workspace_of_a_call(lib):
+    """What a call takes is at most what any call of its sizes does, and less than that
+    is refused; strides and scales that the tensor cores do not take count."""
+    every = lib.gpa_attention_shared_prefix_workspace_bytes
+    for size in [(1, 1, 1, 1, 64, 1, 0), (64, 1, 16, 16, 64, 66845, 1374), (4, 1374, 16, 16, 64, 16711, 1374),
+                 (100, 1, 16, 16, 64, 9000, 33), (16, 17, 8, 8, 128, 9000, 90), (7, 45, 16, 2, 128, 5001, 777),
+                 (3, 515, 16, 8, 128, 4100, 1030), (2, 300, 8, 1, 64, 0, 3000)]:
+        R, M, H, Hk, D, P, N = size
+        for kw in (dict(), dict(scale=-1.0), dict(q_sr=0), dict(q_sr=(M + 1) * H * D)):
+            n = _call_bytes(lib, *size, **kw)
+            assert 0 < n <= every(*size) and n % ((D + 2) * 4) == 0
+    assert _call_bytes(lib, 2, 3, 4, 3, 64, 5, 7) == -1 and _call_bytes(lib, 2, 3, 4, 2, 96, 5, 7) == -1
+    assert _call_bytes(lib, 0, 3, 4, 2, 64, 5, 7) == 0 and _call_bytes(lib, 2, 0, 4, 2, 64, 5, 7) == 0
+    ok = ctypes.c_void_p(256)
+    n = _call_bytes(lib, 4, 1374, 16, 16, 64, 16711, 1374)
+    run = [ok, 1374 * 1024, 64, 1024, ok, 16711 * 64, 64, ok, 16711 * 64, 64, None, 0, ok, 1374 * 1024, 64, 1024, ok,
+           1374 * 1024, 64, 1024, None, None, 4, 1374, 16, 16, 64, 16711, 1374, 0.125, 0, ok, 1374 * 1024, 64, 1024,
+           None, 0, 0, ok, n - 16, None, None]
+    assert lib.gpa_attention_shared_prefix(*run) == 1 and b"workspace" in lib.gpa_last_error()

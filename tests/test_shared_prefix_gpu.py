@@ -558,3 +558,37 @@ def test_exact_scores_that_move_the_maximum(size, scale):
         check(a)
         a["bias"].fill_(-INF)                   # the caches alone, some of them empty
         check(a)
+
+
+@pytest.mark.parametrize("size", EVERY_KERNEL + [(7, 45, 16, 2, 128, 5001, 777), (40, 9, 16, 16, 64, 30000, 600)])
+def test_whatever_the_workspace_holds(size):
+    """Nothing of a workspace is read before the call has written it."""
+    R, M, N = size[0], size[1], size[6]
+    a = make(*size, bias="key", own_len=[(91 * r) % (N + 1) for r in range(R)],
+             q_len=[(53 * r + M) % (M + 1) for r in range(R)], causal=True, seed=41)
+    want = run(a)
+    for value in (float("nan"), 3.0e38, -1.0):
+        torch.cuda.synchronize()
+        held = [torch.full((1 << n,), value, device="cuda") for n in range(10, 25)]
+        del held                               # the allocator hands it to the call
+        got = run(a)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_memory_of_a_large_call():
+    """64 frames of 1,374 tokens: 180 MB of output, and beside it what the cut items
+    leave (20 MB) and 24 bytes a row, not copies of every row."""
+    a = make(64, 1374, 16, 16, 64, 2000, 300, seed=42)
+    _unchecked(a)
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out, lse = _unchecked(a)
+    used = torch.cuda.max_memory_allocated() - before - out.numel() * 2 - lse.numel() * 4
+    assert used < 64 << 20, used
+    r, h = 63, 15                               # the last rows, against the same request alone
+    one = {k: v[r:r + 1] if k in ("q", "k_own", "v_own") else v for k, v in a.items()}
+    ref = reference({**one, "q": one["q"][:, h:], "k_prefix": a["k_prefix"][h:], "v_prefix": a["v_prefix"][h:],
+                     "k_own": one["k_own"][:, h:], "v_own": one["v_own"][:, h:]})
+    off = (out[r:, h:].double() - ref[0]).abs() / (H8 * (ref[0].abs() + ref[1]) + 2.0 ** -10 * ref[1] + 1e-30)
+    assert bool((off <= 1).all())

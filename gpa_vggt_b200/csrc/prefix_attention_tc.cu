@@ -95,7 +95,10 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2 of 8 exponentials on the FMA pipe, the rest on MUFU
+// 2 of 8 exponentials on the FMA pipe, the rest on MUFU.  The cubic is off by up to
+// 7.7e-5: fifty times less than P's rounding to bf16, but the row sum carries it, so
+// lse is off by up to 1.1e-4 where such a key dominates.  Weights below 2^-126 count
+// as that in these two.
 __device__ __forceinline__ void exp8(const float* x, float* e) {
 #pragma unroll
   for (int i = 0; i < 6; ++i) e[i] = fast_exp2(x[i]);

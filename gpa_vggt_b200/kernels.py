@@ -576,7 +576,9 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     count as at most 1e30 either way.  causal: query i sees own keys j <= own_len - q_len + i, and every prefix key.
 
     Returns out [R,H,M,D] bf16, and with return_lse (or lse_out) the log2 row
-    sums [R,H,M] fp32.  A query without keys gives 0 and -inf.  Rows past q_len
+    sums [R,H,M] fp32: to 2^-13 beside the scores' own rounding (a quarter of the
+    tensor cores' exponentials is a cubic), the probabilities of the output to
+    bf16.  A query without keys gives 0 and -inf.  Rows past q_len
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
     -inf.  `out` and `lse_out` lie outside the inputs' memory.  Nothing is read back to the host, so calls can be captured; no
     gradients, backward or forward-mode.  Many rows per key head run on the tensor cores, few as a stream of

@@ -592,3 +592,24 @@ def test_memory_of_a_large_call():
                      "k_own": one["k_own"][:, h:], "v_own": one["v_own"][:, h:]})
     off = (out[r:, h:].double() - ref[0]).abs() / (H8 * (ref[0].abs() + ref[1]) + 2.0 ** -10 * ref[1] + 1e-30)
     assert bool((off <= 1).all())
+
+
+@pytest.mark.parametrize("size", EVERY_KERNEL)
+def test_accuracy_of_the_sums(size):
+    """Rows of two keys with exact scores, the second up to 2^8 times the first, on every
+    lane of a tile: the log2 sum is within 2^-13, more than log2(1 + 7.7e-5) = 1.11e-4
+    of the cubic, and a few roundings of sums below 16."""
+    R, M, H, Hk, D, P, N = size
+    g = torch.Generator(device="cuda").manual_seed(51)
+    for j in list(range(128, 136)) + [3, 255]:
+        a = make(*size, bias="key", own_len=[0] * R, seed=52)
+        a["q"].zero_()
+        a["q"][..., 0] = (torch.rand(R, H, M, device="cuda", generator=g) * 44).bfloat16()
+        a["k_prefix"].zero_()
+        a["k_prefix"][:, j, 0] = 1
+        a["sm_scale"] = 0.125
+        a["bias"].fill_(-INF)
+        a["bias"][[0, j]] = 0
+        _, lse = run(a)
+        ref = torch.log2(1 + torch.exp(a["q"][..., 0].double() * 0.125))
+        assert float((lse.double() - ref).abs().max()) <= 2.0 ** -13 + 2.0 ** -20

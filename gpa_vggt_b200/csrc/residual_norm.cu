@@ -13,8 +13,8 @@
 // a norm of the branch, gate * y is rounded to the stream's type before the add.
 // For a bf16 stream these are the roundings of residual_scale followed by
 // layernorm (norm.cu), so a block that changes from the two kernels to this one
-// keeps its results bit for bit (up to 2,048 columns, where the sums also run in
-// the same order).
+// keeps its results bit for bit (at layernorm's widths up to 2,048 columns, where
+// the sums also run in the same order).
 #include "common.cuh"
 #include "capi_util.h"
 
@@ -517,7 +517,8 @@ static Split split_rows(int64_t rows, int cols, int64_t gate_rows) {
   s.wpr = 1;
   while (s.wpr * s.vpt * 256 < cols) s.wpr *= 2;
   const int64_t groups = rows / gate_rows;
-  // resident workers: 16 warps per SM
+  // 16 warps per SM.  (With a branch norm up to 512 columns, and fp32/fp32 up to 1,024,
+  // the kernel's 143-165 registers let 12 be resident: the last workers run behind.)
   const int64_t most = std::max<int64_t>(148ll * 16 / s.wpr, 1);
   s.whole = groups >= most;
   if (s.whole) {
@@ -547,18 +548,27 @@ static bool kind_ok(int k) { return k == kNone || k == kLayer || k == kRms; }
 template <typename TX, typename TY>
 static int launch_fwd(const FwdParams& p, cudaStream_t st) {
   const int vec = p.cols / 8;
-#define GPA_RN(V, W) fwd_kernel<V, W, TX, TY><<<(unsigned)((p.rows + 8 / W - 1) / (8 / W)), 256, 0, st>>>(p)
-  // few vectors per lane where a vector is many registers (fp32) or waits for many sums
-  const bool order = sizeof(TX) == 2 && p.post_kind == kNone, wide = sizeof(TY) == 4;
-  if (vec <= 32) GPA_RN(1, 1);
-  else if (vec <= 64) GPA_RN(2, 1);
-  else if (vec <= 128 && !wide) GPA_RN(4, 1);
-  else if (vec <= 128) GPA_RN(2, 2);
-  else if (vec <= 256 && order) GPA_RN(8, 1);
-  else if (vec <= 256 && !wide) GPA_RN(4, 2);
-  else if (vec <= 256) GPA_RN(2, 4);
-  else if (vec <= 512) GPA_RN(2, 8);
-  else GPA_RN(4, 8);
+#define GPA_RN(V, W) fwd_kernel<V, W, TX, TY><<<(unsigned)(((int64_t)p.rows + 8 / W - 1) / (8 / W)), 256, 0, st>>>(p)
+  if (vec <= 32) {
+    GPA_RN(1, 1);
+  } else if (vec <= 64) {
+    GPA_RN(2, 1);
+  } else if (vec > 256) {
+    if (vec <= 512) GPA_RN(2, 8);
+    else GPA_RN(4, 8);
+  } else if constexpr (sizeof(TY) == 4) {   // few vectors per lane where a vector is many registers
+    if (vec <= 128) GPA_RN(2, 2);
+    else GPA_RN(2, 4);
+  } else if (vec <= 128) {
+    GPA_RN(4, 1);
+  } else {
+    if constexpr (sizeof(TX) == 2)
+      if (p.post_kind == kNone) {   // layernorm's order of sums
+        GPA_RN(8, 1);
+        return check_launch("gpa_residual_norm");
+      }
+    GPA_RN(4, 2);   // or where it waits for many sums
+  }
 #undef GPA_RN
   return check_launch("gpa_residual_norm");
 }

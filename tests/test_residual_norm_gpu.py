@@ -452,3 +452,31 @@ def test_block_with_a_gamma_of_more_dims(shape):
         ref = block(x)
         block.ls1.gamma = torch.nn.Parameter(block.ls1.gamma.reshape(shape))
         assert torch.equal(block(x), ref)
+
+
+def test_two_steps_at_once():
+    """Training steps on two streams from two threads: the bits that each has alone."""
+    import threading
+    forms = [((3, 900, 1024), BF16, BF16, BF16, "first", "layer", None), ((7, 400, 264), F32, BF16, F32, "token", "rms", "layer"),
+             ((1, 3000, 2048), F32, F32, F32, "channel", "layer", "rms")]
+    cases = [(make(*f, seed=i), train(f[5], f[6])) for i, f in enumerate(forms)]
+    want = [run(dict(t)) for t, run in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def some(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(6):
+                for t, run in cases:
+                    got[i].append(run(dict(t)))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=some, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs in got:
+        assert len(outs) == 18
+        for k, (z, h, grads) in enumerate(outs):
+            wz, wh, wg = want[k % 3]
+            assert torch.equal(z, wz) and torch.equal(h, wh) and all(torch.equal(grads[n], wg[n]) for n in wg)

@@ -613,3 +613,38 @@ def test_accuracy_of_the_sums(size):
         _, lse = run(a)
         ref = torch.log2(1 + torch.exp(a["q"][..., 0].double() * 0.125))
         assert float((lse.double() - ref).abs().max()) <= 2.0 ** -13 + 2.0 ** -20
+
+
+def test_two_calls_at_once():
+    """Calls of every kernel on two streams with nothing between them, and from two
+    threads: each has its own workspace, and the bits it has alone."""
+    import threading
+    cases = [make(*size, bias="key", own_len=[size[6] // (r + 1) for r in range(size[0])], causal=True, seed=61 + i)
+             for i, size in enumerate(EVERY_KERNEL)]
+    want = [run(a) for a in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def some(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(3):
+                for a in cases[::-1] if i else cases:
+                    got[i].append(_unchecked(a))
+
+    for _ in range(2):                          # interleaved by hand, then by the threads
+        for a, b in zip(cases, cases[::-1]):
+            for i, c in ((0, a), (1, b)):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(_unchecked(c))
+    threads = [threading.Thread(target=some, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert len(outs) == 5 * len(cases)
+        for k, (o, lse) in enumerate(outs):
+            w = want[::-1][k % len(cases)] if i else want[k % len(cases)]
+            assert torch.equal(o, w[0]) and torch.equal(lse, w[1])

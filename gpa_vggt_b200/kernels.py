@@ -466,16 +466,23 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[
 
 
 def _vectors(t: torch.Tensor):
-    """(t or a copy of it, strides of all dims but the last, 0 where a dim has at
-    most one entry: what stands there says nothing, also where t counts as
-    contiguous): innermost dim contiguous, 16-byte aligned vectors."""
-    if t.numel() == 0:
-        return t, (0,) * (t.dim() - 1)
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    if t.stride(-1) != 1 or not aligned(t) or any(s % 8 for s in strides[:-1]):
+    """(t or a copy of it, strides of all dims but the last, those that say something
+    multiples of 8 and the others 0 or that): innermost dim contiguous, 16-byte
+    aligned vectors."""
+    strides = t.stride()[:-1]
+    whole = t.is_contiguous() and aligned(t)
+    if whole:
+        odd = 0
+        for s in strides:
+            odd |= s
+        if not odd & 7:
+            return t, strides
+    # a dim with at most one entry, or an empty tensor, may have any stride
+    strides = [s if n > 1 else 0 for s, n in zip(strides, t.shape)] if t.numel() else [0] * len(strides)
+    if not whole and (t.stride(-1) != 1 or not aligned(t) or any(s % 8 for s in strides)):
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    return t, strides[:-1]
+        strides = t.stride()[:-1]
+    return t, strides
 
 
 def _span(t: torch.Tensor):
@@ -609,8 +616,10 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         if bias.dim() == 2 and bias.shape[0] > 1:
             bias_sh = bias.stride(0)
     own_len, q_len = (None if t is None else t.contiguous() for t in (own_len, q_len))
-    size = _lib.load().gpa_attention_shared_prefix_call_bytes(*qs, *kps, *vps, *kos, *vos, R, M, H, Hk, D, P, N,
-                                                              sm_scale)
+    lib = _lib.load()
+    size = lib.gpa_attention_shared_prefix_workspace_bytes(R, M, H, Hk, D, P, N)
+    if size > 1 << 26:   # enough for any strides; what these take costs 4 us to ask
+        size = lib.gpa_attention_shared_prefix_call_bytes(*qs, *kps, *vps, *kos, *vos, R, M, H, Hk, D, P, N, sm_scale)
     ws = torch.empty(size, device=device, dtype=torch.uint8) if size > 0 else None
     status, own = _status_word(status, device)
     ls = (0, 0) if lse_out is None else lse_out.stride()[:2]

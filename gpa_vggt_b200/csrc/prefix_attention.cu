@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 32) join_kernel(const Param
 // Joins tc_kernel's parts (and rows_kernel's chunks of the caches, in a folded
 // call): a thread per row of a 128-row tile, F features of it.  FEW tiles are cut
 // into many parts, and the time is the latency of their loads in turn: 8 features a
-// thread and 8 parts in flight hide it (128 rows over 66,845 keys: 77 us with
+// thread and 8 parts in flight hide it (128 rows over 66,845 keys: 77-80 us with
 // tc_kernel, 85 with 32 features and a part at a time; 7 requests of 45 tokens: 41
 // and 48).  Many tiles fill the GPU with 32 features, in longer runs of a row (3 x
 // 515 tokens: 107 us, 112 with 8; 8 x 300 over 8,191 + 1,030 keys: 191 and 204).

@@ -28,13 +28,13 @@
 // waits for O += P(j) V; the other stream's softmax runs meanwhile.
 //
 // Bound by the softmax at head_dim 64 (issue slots and MUFU: 50% and 55% busy, the
-// tensor pipe 45%) and by the issuers' round trip at 128.  Whole tiles (9,472 rows
-// x 16,384 keys, by card and power): 840-855 TFLOP/s for 16 heads of 64 (806-834
-// with a bias), 950-1,095 for 8 of 128.  Four requests of 1,374 tokens over 16,711
-// + 1,374 keys: 540 us (one CTA per item 685: 384 items end in a third of a wave).
-// In halves 64 rows over 66,845 keys take 76 us with the join, 128 rows 77: 7 us
-// until the first scores, then 1.95 a key tile and stream (77% of the measured copy
-// rate).
+// tensor pipe 40%) and by the issuers' round trip at 128.  Whole tiles (9,472 rows
+// x 16,384 keys, replayed from a graph, by card and power): 840-865 TFLOP/s for 16
+// heads of 64 (780-834 with a bias), 930-1,095 for 8 of 128.  Four requests of 1,374
+// tokens over 16,711 + 1,374 keys: 540-550 us (one CTA per item 685: 384 items end in
+// a third of a wave).  In halves 64 rows over 66,845 keys take 76-79 us with the join,
+// 128 rows 77-80: 7 us until the first scores, then 1.95 a key tile and stream (77%
+// of the measured copy rate).
 #include "prefix_attention.cuh"
 
 namespace gpa {

@@ -385,8 +385,7 @@ GPA_API int gpa_gelu_bf16(const void* x, int64_t n, void* out, void* stream);
 
 /*
  * Gated residual with the norms around it (the residual adds, LayerScales and
- * norms of vggt/layers/block.py:85-94 and layer_scale.py:21; the gate of
- * vggt/heads/camera_head.py), one pass:
+ * norms of vggt/layers/block.py:85-94 and layer_scale.py:21), one pass:
  *   z[r] = x[r] + gate[r / gate_rows] * P(y[r]),   h[r] = N(z[r])
  * P: post_kind GPA_NORM_NONE (y itself), _LAYER or _RMS with optional
  * post_weight / post_bias; N: kind likewise with weight / bias (GPA_NORM_NONE:

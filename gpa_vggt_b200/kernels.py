@@ -133,7 +133,7 @@ def _one_device(first: torch.Tensor, *others, what: str) -> int:
 def has_tangent(*tensors) -> bool:
     """Whether one of them carries a forward-mode derivative, which a kernel that
     works on addresses would drop without a word."""
-    return forward_ad._current_level >= 0 and any(
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
@@ -580,16 +580,18 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     on the device (clamped to [0,N] and [0,M]), or None for all N and M; cache
     rows past own_len may hold anything.  bias: [P], [1,P] or [Hk,P], natural-log
     domain; -inf (or NaN) takes a key out, whatever its K and V hold; finite ones
-    count as at most 1e30 either way.  causal: query i sees own keys j <= own_len - q_len + i, and every prefix key.
+    count as at most 1e30 either way.  causal: query i sees own keys
+    j <= own_len - q_len + i, and every prefix key.
 
     Returns out [R,H,M,D] bf16, and with return_lse (or lse_out) the log2 row
     sums [R,H,M] fp32: to 2^-13 beside the scores' own rounding (a quarter of the
     tensor cores' exponentials is a cubic), the probabilities of the output to
     bf16.  A query without keys gives 0 and -inf.  Rows past q_len
     are left as they were in `out` / `lse_out`; in fresh outputs they are 0 and
-    -inf.  `out` and `lse_out` lie outside the inputs' memory.  Nothing is read back to the host, so calls can be captured; no
-    gradients, backward or forward-mode.  Many rows per key head run on the tensor cores, few as a stream of
-    the keys (the choice is by sizes and strides, not by values); a pipeline wait
+    -inf.  `out` and `lse_out` lie outside the inputs' memory (also between an
+    input's rows).  Nothing is read back to the host, so calls can be captured; no
+    gradients, backward or forward-mode.  Many rows per key head run on the tensor
+    cores, few as a stream of the keys (the choice is by sizes and strides, not by values); a pipeline wait
     that gives up is recorded in the device's status word (check_device_status)."""
     index = _check_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, bias, out, lse_out, status)
     R, H, M, D = q.shape

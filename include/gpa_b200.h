@@ -445,9 +445,10 @@ GPA_API int gpa_residual_norm_backward(
  * + i (the last query sees all); the prefix is seen by every query.  A query
  * without keys gives 0 and lse -inf.  lse: fp32 (to 2^-13 beside the scores'
  * rounding), rows contiguous, or NULL.  o and lse overlap no input.  status:
- * device int, set to 1 where a pipeline wait gives up, or NULL.  workspace: 16-byte aligned; calls that may overlap need their
- * own.  _workspace_bytes() is enough for any strides and scale, _call_bytes() for a
- * call with these (-1: bad sizes).
+ * device int, set to 1 where a pipeline wait gives up, or NULL.  workspace:
+ * 16-byte aligned; calls that may overlap need their own.  _workspace_bytes() is
+ * enough for any strides and scale, _call_bytes() for a call with these (-1: bad
+ * sizes).
  */
 GPA_API int64_t gpa_attention_shared_prefix_workspace_bytes(int requests, int queries, int heads, int kv_heads,
                                                             int head_dim, int prefix, int cache);

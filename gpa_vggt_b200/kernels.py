@@ -612,7 +612,10 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     os = _vectors(out)[1]
     bias_sh = 0
     if bias is not None:
-        bias = bias.detach().to(F32)
+        bias = bias.detach()
+        if bias.dtype == torch.float64:   # finite values beyond fp32's stay finite
+            bias = torch.where(bias > -float("inf"), bias.clamp(-1e30, 1e30), bias)
+        bias = bias.to(F32)
         if P > 1 and bias.stride(-1) != 1:
             bias = bias.contiguous()
         if bias.dim() == 2 and bias.shape[0] > 1:

@@ -648,3 +648,23 @@ def test_two_calls_at_once():
         for k, (o, lse) in enumerate(outs):
             w = want[::-1][k % len(cases)] if i else want[k % len(cases)]
             assert torch.equal(o, w[0]) and torch.equal(lse, w[1])
+
+
+@pytest.mark.parametrize("M", [1, 260])
+@pytest.mark.parametrize("dtype", [torch.float16, BF16, F32, F64])
+def test_lowest_bias_of_every_type(M, dtype):
+    """A row of nothing but the type's lowest value spreads evenly; beside another key
+    it counts for nothing, and -inf (or NaN) takes a key out."""
+    a = make(3, M, 4, 4, 64, 3000, 40, own_len=[0] * 3, seed=71)
+    a["q"].zero_()
+    a["bias"] = torch.full((4, 3000), torch.finfo(dtype).min, device="cuda", dtype=dtype)
+    o, lse = run(a)
+    v = a["v_prefix"].double()
+    mean, mag = v.mean(1)[None, :, None], v.abs().mean(1)[None, :, None]
+    assert bool(((o.double() - mean).abs() <= H8 * (mean.abs() + mag) + 2.0 ** -10 * mag).all())
+    assert bool(torch.isfinite(lse).all())
+    a["bias"][:, 1000:] = -INF
+    a["bias"][:, 1500] = float("nan")
+    a["bias"][:, 77] = torch.finfo(dtype).max if dtype != torch.float16 else 0
+    o, _ = run(a)
+    assert torch.equal(o, a["v_prefix"][:, 77][None, :, None].expand_as(o))

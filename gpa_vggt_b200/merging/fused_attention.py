@@ -54,7 +54,9 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     if q.dtype == torch.float32:
         dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else torch.bfloat16
         q, k_prefix, v_prefix, k_own, v_own = (t.to(dt) for t in (q, k_prefix, v_prefix, k_own, v_own))
-        bias = None if bias is None else bias.to(dt)
+        if bias is not None:   # fp32's lowest value would round to -inf, which takes a key out
+            most = torch.finfo(dt).max
+            bias = torch.where(bias > -float("inf"), bias.clamp(-most, most), bias).to(dt)
     if q.dtype == torch.float16:
         raise NotImplementedError("attention_shared_prefix: fp16 inputs are not supported (bf16 only)")
     return kernels.attention_shared_prefix(q, k_prefix, v_prefix, k_own, v_own, sm_scale, own_len=own_len,

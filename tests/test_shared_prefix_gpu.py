@@ -668,3 +668,17 @@ def test_lowest_bias_of_every_type(M, dtype):
     a["bias"][:, 77] = torch.finfo(dtype).max if dtype != torch.float16 else 0
     o, _ = run(a)
     assert torch.equal(o, a["v_prefix"][:, 77][None, :, None].expand_as(o))
+
+
+def test_public_form_keeps_the_lowest_bias_finite():
+    """fp32's lowest value stays a weight when the public form casts to bf16."""
+    from gpa_vggt_b200.merging import attention_shared_prefix
+    a = make(2, 5, 4, 2, 64, 90, 40, own_len=[0, 0])
+    a["q"].zero_()
+    f = {k: a[k].float() for k in ("q", "k_prefix", "v_prefix", "k_own", "v_own")}
+    bias = torch.full((90,), torch.finfo(F32).min, device="cuda")
+    bias[30:] = -INF
+    o = attention_shared_prefix(*f.values(), bias, 0.125, own_len=a["own_len"])
+    v = a["v_prefix"][:, :30].double().repeat_interleave(2, 0)
+    mean, mag = v.mean(1)[None, :, None], v.abs().mean(1)[None, :, None]
+    assert bool(((o.double() - mean).abs() <= H8 * (mean.abs() + mag) + 2.0 ** -10 * mag).all())
